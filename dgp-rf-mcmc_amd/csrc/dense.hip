@@ -1,0 +1,717 @@
+// dense.hip — the dense operators' entry points (dgprf_linear_forward / _backward, dgprf_dropout),
+// the rules that choose their kernels, and the kernels around the tiled product (dense_gemm_impl.h).
+#include <algorithm>
+#include <cmath>
+
+#include "dense_common.h"
+
+using namespace dense;
+
+namespace {
+
+inline int64_t up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
+inline int64_t cdiv(int64_t x, int64_t m) { return (x + m - 1) / m; }
+
+// ---------------------------------------------------------------- packing
+// Rows of `cols` elements at any stride and alignment to rows of ldo, zero-padded: the tiled product
+// reads 16 bytes at a time.
+template <class T>
+__global__ __launch_bounds__(256) void k_pack(const T* __restrict__ in, int64_t ld, int rows, int cols,
+                                              T* __restrict__ out, int ldo) {
+  const int per = ldo >> 3;  // ldo % 8 == 0
+  const int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (q >= (int64_t)rows * per) return;
+  const int64_t row = q / per;
+  const int col = (int)(q - row * per) * 8;
+  const T* p = in + row * ld;
+  typename Vec<T>::v8 v;
+#pragma unroll
+  for (int c = 0; c < 8; ++c) v[c] = col + c < cols ? p[col + c] : (T)0.f;
+  *reinterpret_cast<typename Vec<T>::v8*>(out + row * ldo + col) = v;
+}
+
+// ---------------------------------------------------------------- eight columns of a row
+struct F8 {
+  f4 lo, hi;
+};
+template <class T>
+__device__ __forceinline__ F8 load8(const T* row, int col, int n, bool aligned) {
+  F8 v;
+  if (aligned && col + 8 <= n) {
+    const typename Vec<T>::v8 x = *reinterpret_cast<const typename Vec<T>::v8*>(row + col);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      v.lo[c] = (float)x[c];
+      v.hi[c] = (float)x[c + 4];
+    }
+  } else {
+    v.lo = load4_edge(row, col, n, false);
+    v.hi = load4_edge(row, col + 4, n, false);
+  }
+  return v;
+}
+template <class T>
+__device__ __forceinline__ void store8(T* row, int col, int n, bool aligned, F8 v) {
+  if (aligned && col + 8 <= n) {
+    typename Vec<T>::v8 x;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      x[c] = (T)v.lo[c];
+      x[c + 4] = (T)v.hi[c];
+    }
+    *reinterpret_cast<typename Vec<T>::v8*>(row + col) = x;
+  } else {
+    store4_edge(row, col, n, false, v.lo);
+    store4_edge(row, col + 4, n, false, v.hi);
+  }
+}
+__device__ __forceinline__ F8 drop8(F8 v, const u32x4& w, const DropDev& d) {
+  v.lo[0] = drop_lo(v.lo[0], w.x, d);
+  v.lo[1] = drop_hi(v.lo[1], w.x, d);
+  v.lo[2] = drop_lo(v.lo[2], w.y, d);
+  v.lo[3] = drop_hi(v.lo[3], w.y, d);
+  v.hi[0] = drop_lo(v.hi[0], w.z, d);
+  v.hi[1] = drop_hi(v.hi[1], w.z, d);
+  v.hi[2] = drop_lo(v.hi[2], w.w, d);
+  v.hi[3] = drop_hi(v.hi[3], w.w, d);
+  return v;
+}
+
+// ---------------------------------------------------------------- joining the parts of K
+// Sums the parts in order (so a result does not depend on which part was ready first) and applies the
+// epilogue; one thread for eight columns of a row.  e.y 8-aligned rows: vec.
+template <class T>
+__global__ __launch_bounds__(256) void k_join(const float* __restrict__ part, int64_t ldp, int parts,
+                                              int64_t rows, const EpiDev e) {
+  const int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (q >= rows * e.groups) return;
+  const int64_t row = q / e.groups;
+  const int col = (int)(q - row * e.groups) * 8, n = e.n;
+  const float* p = part + row * ldp + col;
+  const int64_t stride = rows * ldp;
+  F8 v;
+  v.lo = f4zero();
+  v.hi = f4zero();
+  const bool hi = col + 4 < ldp;  // ldp % 4 == 0
+  for (int s = 0; s < parts; ++s, p += stride) {
+    v.lo += *reinterpret_cast<const f4*>(p);
+    if (hi) v.hi += *reinterpret_cast<const f4*>(p + 4);
+  }
+  if (e.bias) {
+    v.lo += load4_edge((const T*)e.bias, col, n, false);
+    v.hi += load4_edge((const T*)e.bias, col + 4, n, false);
+  }
+  if (e.aux || e.act != DGPRF_ACT_NONE) {
+    with_act(e.act, [&](auto act) {
+      constexpr int ACT = decltype(act)::value;
+      F8 z;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        z.lo[c] = saved_of<ACT>(v.lo[c]);
+        z.hi[c] = saved_of<ACT>(v.hi[c]);
+        v.lo[c] = act_of<T, ACT>(v.lo[c]);
+        v.hi[c] = act_of<T, ACT>(v.hi[c]);
+      }
+      if (e.aux) store8((T*)e.aux + row * e.ldaux, col, (int)e.ldaux, true, z);
+    });
+  }
+  if (e.drop.thr) v = drop8(v, drop_words(e.drop, drop_sub(e.drop), (uint64_t)q), e.drop);
+  if (e.res) {
+    const F8 r = load8((const T*)e.res + row * e.ldr, col, n, e.vec_r == 2);
+    v.lo += r.lo;
+    v.hi += r.hi;
+  }
+  store8((T*)e.y + row * e.ldy, col, n, e.vec_y == 2, v);
+}
+
+// ---------------------------------------------------------------- few rows
+// z = x W for up to MR rows: W is read once, at memory speed, by many workgroups, and each product is
+// a plain multiply-add (2 MR operations a weight; the matrix instructions would pad MR to 16).  A
+// workgroup takes 16 lanes' width of columns and up to 1024 k; its 16 k-lanes (4 of a wave, 4 waves)
+// take groups of four k each, whose x values are one LDS read, and their sums are added in a fixed
+// order.  Parts of K are joined by k_join.
+constexpr int kRowsK = 1024;
+template <class T, int MR, bool VEC>
+__global__ __launch_bounds__(256) void k_rows(const T* __restrict__ x, int64_t ldx,
+                                              const T* __restrict__ w, int64_t ldw, int M, int K, int N,
+                                              int k_part, float* __restrict__ part, int64_t ldp) {
+  constexpr int CE = 16 / (int)sizeof(T), STRIP = 16 * CE;
+  typedef T vec __attribute__((ext_vector_type(CE)));
+  __shared__ __attribute__((aligned(16))) float xs[MR * kRowsK];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int k0 = blockIdx.y * k_part, kn = min(k_part, K - k0), kp = (kn + 3) & ~3;
+  const int col = blockIdx.x * STRIP + (lane & 15) * CE;
+  for (int i = tid; i < MR * kp; i += 256) {
+    const int m = i / kp, k = i - m * kp;
+    xs[m * kRowsK + k] = m < M && k < kn ? (float)x[m * ldx + k0 + k] : 0.f;
+  }
+  __syncthreads();
+  float acc[MR][CE];
+#pragma unroll
+  for (int m = 0; m < MR; ++m)
+#pragma unroll
+    for (int c = 0; c < CE; ++c) acc[m][c] = 0.f;
+  if (col < N) {
+    const T* wp = w + (int64_t)k0 * ldw + col;
+#pragma unroll 2
+    for (int k = (wave * 4 + (lane >> 4)) * 4; k < kn; k += 64) {
+      T v[4][CE];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const T* p = wp + (int64_t)(k + r) * ldw;
+        if constexpr (VEC) {
+          const vec u = k + r < kn ? *reinterpret_cast<const vec*>(p) : (vec)(T)0.f;
+#pragma unroll
+          for (int c = 0; c < CE; ++c) v[r][c] = u[c];
+        } else {
+#pragma unroll
+          for (int c = 0; c < CE; ++c) v[r][c] = k + r < kn && col + c < N ? p[c] : (T)0.f;
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < MR; ++m) {
+        const f4 xv = *reinterpret_cast<const f4*>(&xs[m * kRowsK + k]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int c = 0; c < CE; ++c) acc[m][c] = fmaf(xv[r], (float)v[r][c], acc[m][c]);
+      }
+    }
+  }
+  __syncthreads();
+  // the four k-lanes of a wave, then the four waves
+#pragma unroll
+  for (int m = 0; m < MR; ++m)
+#pragma unroll
+    for (int c = 0; c < CE; ++c) {
+      float s = acc[m][c];
+      s += __shfl_xor(s, 16);
+      s += __shfl_xor(s, 32);
+      if (lane < 16) xs[(wave * MR + m) * STRIP + lane * CE + c] = s;
+    }
+  __syncthreads();
+  float* out = part + (int64_t)blockIdx.y * M * ldp;
+  for (int i = tid; i < MR * STRIP; i += 256) {
+    const int m = i / STRIP, c = i - m * STRIP, j = blockIdx.x * STRIP + c;
+    float s = 0.f;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) s += xs[(v * MR + m) * STRIP + c];
+    if (m < M && j < N) out[m * ldp + j] = s;
+  }
+}
+
+// ---------------------------------------------------------------- dz and its column sums
+// dz = s m dy a'(z) (rounded to the tensors' type, as the matrix instructions take it; its sums for
+// db are of the unrounded values), one thread for eight columns and `rows_part` rows; dz is null
+// where it would equal dy.
+struct DzDev {
+  const void* dy;
+  const void* aux;
+  void* dz;
+  float* part;  // [parts][ldz] or null
+  int64_t lddy, ldaux, ldz;
+  int64_t M;
+  int32_t N, groups, act, vec, rows_part;
+  DropDev drop;
+};
+template <class T>
+__global__ __launch_bounds__(256) void k_dz(const DzDev d) {
+  __shared__ __attribute__((aligned(16))) float sums[4][64 * 8];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int gi = blockIdx.x * 64 + lane, col = gi * 8;
+  const int64_t m0 = (int64_t)blockIdx.y * d.rows_part, m1 = min(d.M, m0 + d.rows_part);
+  const uint64_t sub = d.drop.thr ? drop_sub(d.drop) : 0;
+  F8 acc;
+  acc.lo = f4zero();
+  acc.hi = f4zero();
+  if (gi < d.groups) {
+    with_act(d.act, [&](auto act) {
+      constexpr int ACT = decltype(act)::value;
+      for (int64_t m = m0 + wave; m < m1; m += 4) {
+        F8 v = load8((const T*)d.dy + m * d.lddy, col, d.N, d.vec);
+        if constexpr (ACT != DGPRF_ACT_NONE) {
+          const F8 z = load8((const T*)d.aux + m * d.ldaux, col, (int)d.ldaux, true);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            v.lo[c] *= slope_of<T, ACT>(z.lo[c]);
+            v.hi[c] *= slope_of<T, ACT>(z.hi[c]);
+          }
+        }
+        // last, so that a dropped element is 0 whatever its gradient and slope
+        if (d.drop.thr) v = drop8(v, drop_words(d.drop, sub, (uint64_t)m * (uint32_t)d.groups + (uint32_t)gi), d.drop);
+        // zeros past N: the tiled product multiplies the padding
+        if (d.dz) {
+          if (col + 8 > d.N) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              if (col + c >= d.N) v.lo[c] = 0.f;
+              if (col + 4 + c >= d.N) v.hi[c] = 0.f;
+            }
+          }
+          store8((T*)d.dz + m * d.ldz, col, (int)d.ldz, true, v);
+        }
+        acc.lo += v.lo;
+        acc.hi += v.hi;
+      }
+    });
+  }
+  if (!d.part) return;
+  *reinterpret_cast<f4*>(&sums[wave][lane * 8]) = acc.lo;
+  *reinterpret_cast<f4*>(&sums[wave][lane * 8 + 4]) = acc.hi;
+  __syncthreads();
+  for (int i = threadIdx.x; i < 512; i += 256) {
+    const int c = blockIdx.x * 512 + i;
+    if (c < d.ldz) d.part[(int64_t)blockIdx.y * d.ldz + c] = sums[0][i] + sums[1][i] + sums[2][i] + sums[3][i];
+  }
+}
+
+// db[c] = sum of the parts: 32 columns of a workgroup, eight threads each, in a fixed order
+template <class T>
+__global__ __launch_bounds__(256) void k_db(const float* __restrict__ part, int64_t ldp, int parts, int N,
+                                            T* __restrict__ db) {
+  __shared__ float sums[8][33];
+  const int cl = threadIdx.x & 31, r = threadIdx.x >> 5, c = blockIdx.x * 32 + cl;
+  float s = 0.f;
+  if (c < N)
+    for (int p = r; p < parts; p += 8) s += part[p * ldp + c];
+  sums[r][cl] = s;
+  __syncthreads();
+  if (r == 0 && c < N) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) s += sums[i][cl];
+    db[c] = (T)s;
+  }
+}
+
+// ---------------------------------------------------------------- dropout
+// FLAT: rows without gaps whose length is a multiple of 8: the group's number is its place
+template <class T, bool FLAT>
+__global__ __launch_bounds__(256) void k_dropout(const T* __restrict__ x, int64_t ldx,
+                                                 const T* __restrict__ res, int64_t ldr,
+                                                 T* __restrict__ y, int64_t total, int groups, int n,
+                                                 const DropDev d) {
+  const int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (q >= total) return;
+  const uint64_t sub = drop_sub(d);
+  if constexpr (FLAT) {
+    F8 v = load8(x + 8 * q, 0, 8, true);
+    if (d.thr) v = drop8(v, drop_words(d, sub, (uint64_t)q), d);
+    if (res) {
+      const F8 r = load8(res + 8 * q, 0, 8, true);
+      v.lo += r.lo;
+      v.hi += r.hi;
+    }
+    store8(y + 8 * q, 0, 8, true, v);
+  } else {
+    const int64_t row = q / groups;
+    const int col = (int)(q - row * groups) * 8;
+    F8 v = load8(x + row * ldx, col, n, false);
+    if (d.thr) v = drop8(v, drop_words(d, sub, (uint64_t)q), d);
+    if (res) {
+      const F8 r = load8(res + row * ldr, col, n, false);
+      v.lo += r.lo;
+      v.hi += r.hi;
+    }
+    store8(y + row * (int64_t)n, col, n, false, v);
+  }
+}
+
+// ---------------------------------------------------------------- choices
+bool aligned(const void* p, int64_t ld, int64_t cols, int es, int bytes) {
+  return (uintptr_t)p % bytes == 0 && ld * es % bytes == 0 && cols * es % bytes == 0;
+}
+// rows of 16-byte pieces: what the tiled product reads in place
+bool in_place(const void* p, int64_t ld, int64_t cols, int es) { return aligned(p, ld, cols, es, 16); }
+
+struct Shape {
+  int tile, n_mt, n_nt, splits, stages, stages_split;
+};
+constexpr int kRowsMax = 8;  // rows the streaming kernel takes
+constexpr int64_t kMaxWidth = 1 << 20;  // a tile's rows stay within a buffer descriptor's range
+
+// Tile and parts of K for an I x J result.
+Shape shape_of(int64_t I, int64_t J, int64_t K, int es) {
+  Shape s;
+  const int64_t big = cdiv(I, 256) * cdiv(J, 256);
+  s.tile = I <= 32 ? TILE_32 : big >= 160 ? TILE_256 : TILE_128;
+  const int bm = s.tile == TILE_256 ? 256 : s.tile == TILE_128 ? 128 : 32, bn = s.tile == TILE_256 ? 256 : 128;
+  s.n_mt = (int)cdiv(I, bm);
+  s.n_nt = (int)cdiv(J, bn);
+  s.stages = (int)cdiv(K * es, 128);
+  const int64_t tiles = (int64_t)s.n_mt * s.n_nt;
+  int64_t want = tiles < 256 ? cdiv(512, tiles) : 1;
+  want = std::min<int64_t>({want, std::max(1, s.stages / 4), 32});
+  s.stages_split = (int)cdiv(s.stages, want);
+  s.splits = (int)cdiv(s.stages, s.stages_split);
+  return s;
+}
+int64_t part_bytes(const Shape& s, int64_t I, int64_t J) {
+  return s.splits > 1 ? up((int64_t)s.splits * I * up(J, 4) * 4, 256) : 0;
+}
+
+// parts of K for the few-row kernel: enough workgroups to keep the memory busy
+void rows_shape(int64_t N, int64_t K, int es, int* k_part, int* parts) {
+  const int64_t strips = cdiv(N, 256 / es);
+  int64_t p = std::max<int64_t>(cdiv(K, kRowsK), std::min<int64_t>(cdiv(1024, strips), cdiv(K, 64)));
+  *k_part = (int)up(cdiv(K, p), 4);
+  *parts = (int)cdiv(K, *k_part);
+}
+
+struct Scratch {  // a bump allocator over the caller's scratch; base null: only counts
+  char* base;
+  int64_t used = 0;
+  void* take(int64_t bytes) {
+    void* p = base ? base + used : nullptr;
+    used += up(bytes, 256);
+    return p;
+  }
+};
+
+DropDev drop_dev(int32_t thr, uint64_t seed, uint64_t sub, const int64_t* step) {
+  DropDev d;
+  d.thr = (uint32_t)thr;
+  d.scale = thr < 65536 ? 65536.f / (float)(65536 - thr) : 0.f;
+  d.k0 = (uint32_t)seed;
+  d.k1 = (uint32_t)(seed >> 32);
+  d.sub = sub;
+  d.step = step;
+  return d;
+}
+
+hipError_t gemm(int dtype, int layout, const Shape& s, const GemmArgs& a, const EpiDev& e, hipStream_t st) {
+  if (dtype == DGPRF_BF16) return launch_gemm_bf16(layout, s.tile, a, e, st);
+  if (dtype == DGPRF_F16) return launch_gemm_f16(layout, s.tile, a, e, st);
+  return launch_gemm_f32(layout, s.tile, a, e, st);
+}
+
+// f((T*)nullptr) for the element type
+template <class F>
+hipError_t with_type(int dtype, F f) {
+  if (dtype == DGPRF_BF16) return f((bf16_t*)nullptr);
+  if (dtype == DGPRF_F16) return f((f16_t*)nullptr);
+  return f((float*)nullptr);
+}
+#define DENSE_T(p) typename std::remove_pointer<decltype(p)>::type
+
+hipError_t pack(int dtype, const void* in, int64_t ld, int64_t rows, int64_t cols, void* out, hipStream_t s) {
+  const int64_t ldo = up(cols, 8), q = rows * (ldo / 8);
+  return with_type(dtype, [&](auto* t) {
+    typedef DENSE_T(t) T;
+    hipLaunchKernelGGL((k_pack<T>), dim3((unsigned)cdiv(q, 256)), dim3(256), 0, s, (const T*)in, ld, (int)rows,
+                       (int)cols, (T*)out, (int)ldo);
+    return hipGetLastError();
+  });
+}
+
+hipError_t join(int dtype, const float* part, int64_t ldp, int parts, int64_t rows, const EpiDev& e,
+                hipStream_t s) {
+  return with_type(dtype, [&](auto* t) {
+    typedef DENSE_T(t) T;
+    hipLaunchKernelGGL((k_join<T>), dim3((unsigned)cdiv(rows * e.groups, 256)), dim3(256), 0, s, part, ldp,
+                       parts, rows, e);
+    return hipGetLastError();
+  });
+}
+
+template <class T, int MR>
+hipError_t rows_launch(const dgprf_linear_t& a, bool vec, int k_part, int parts, float* part, int64_t ldp,
+                       hipStream_t s) {
+  const dim3 grid((unsigned)cdiv(a.n, 256 / (int)sizeof(T)), (unsigned)parts);
+  if (vec)
+    hipLaunchKernelGGL((k_rows<T, MR, true>), grid, dim3(256), 0, s, (const T*)a.x, a.ldx, (const T*)a.w, a.ldw,
+                       (int)a.m, (int)a.k, (int)a.n, k_part, part, ldp);
+  else
+    hipLaunchKernelGGL((k_rows<T, MR, false>), grid, dim3(256), 0, s, (const T*)a.x, a.ldx, (const T*)a.w, a.ldw,
+                       (int)a.m, (int)a.k, (int)a.n, k_part, part, ldp);
+  return hipGetLastError();
+}
+
+// One product of the layer: [I][J] over K into scratch parts or straight through the epilogue.
+hipError_t product(int dtype, int layout, const void* A, int64_t lda, const void* B, int64_t ldb, int64_t I,
+                   int64_t J, int64_t Ia, int64_t Ja, int64_t Ka, int64_t Kb, const EpiDev& e, Scratch& sc,
+                   hipStream_t st, bool run) {
+  const int es = elem_size(dtype);
+  const Shape s = shape_of(I, J, std::max(Ka, Kb), es);
+  float* part = (float*)sc.take(part_bytes(s, I, J));
+  if (!run) return hipSuccess;
+  GemmArgs a;
+  a.A = A;
+  a.B = B;
+  a.lda = lda;
+  a.ldb = ldb;
+  a.I = (int)I;
+  a.J = (int)J;
+  a.Ia = (int)Ia;
+  a.Ja = (int)Ja;
+  a.Ka = (int)Ka;
+  a.Kb = (int)Kb;
+  a.n_mt = s.n_mt;
+  a.n_nt = s.n_nt;
+  a.splits = s.splits;
+  a.stages = s.stages;
+  a.stages_split = s.stages_split;
+  a.part = s.splits > 1 ? part : nullptr;
+  a.ldp = up(J, 4);
+  hipError_t err = gemm(dtype, layout, s, a, e, st);
+  if (err == hipSuccess && a.part) err = join(dtype, part, a.ldp, s.splits, I, e, st);
+  return err;
+}
+
+EpiDev epi_plain(void* y, int64_t n, int es) {
+  EpiDev e{};
+  e.y = y;
+  e.ldy = n;
+  e.n = (int)n;
+  e.groups = (int)cdiv(n, 8);
+  e.vec_y = aligned(y, n, n, es, 8 * es) ? 2 : aligned(y, n, n, es, 4 * es) ? 1 : 0;
+  return e;
+}
+
+int check_drop(int32_t thr) { return thr < 0 || thr > 65536 ? DGPRF_E_ARG : DGPRF_OK; }
+
+int check_dims(int32_t dtype, int32_t act, int64_t m, int64_t k, int64_t n, int64_t ldx, int64_t ldw) {
+  if (dtype != DGPRF_F32 && dtype != DGPRF_F16 && dtype != DGPRF_BF16) return DGPRF_E_ARG;
+  if (act < DGPRF_ACT_NONE || act > DGPRF_ACT_SILU) return DGPRF_E_ARG;
+  if (m < 0 || k < 1 || n < 1 || ldx < k || ldw < n) return DGPRF_E_SHAPE;
+  if (m >= ((int64_t)1 << 31) || k > kMaxWidth || n > kMaxWidth || ldx > kMaxWidth || ldw > kMaxWidth)
+    return DGPRF_E_SHAPE;
+  // workgroups of the per-eight-columns kernels
+  if (m * cdiv(std::max(k, n), 8) >= ((int64_t)1 << 39)) return DGPRF_E_SHAPE;
+  return DGPRF_OK;
+}
+
+// The forward pass; run = false only counts its scratch.
+hipError_t forward(const dgprf_linear_t& a, Scratch& sc, hipStream_t st, bool run) {
+  const int es = elem_size(a.dtype);
+  const int64_t m = a.m, k = a.k, n = a.n;
+  EpiDev e = epi_plain(a.y, n, es);
+  e.bias = a.bias;
+  e.res = a.res;
+  e.aux = a.act != DGPRF_ACT_NONE ? a.aux : nullptr;
+  e.ldr = a.ldr;
+  e.ldaux = up(n, 8);
+  e.act = a.act;
+  e.vec_r = aligned(a.res, a.ldr, 0, es, 8 * es) ? 2 : aligned(a.res, a.ldr, 0, es, 4 * es) ? 1 : 0;
+  e.drop = drop_dev(a.drop_thr, a.seed, a.sub, a.step);
+  if (m <= kRowsMax) {
+    int k_part, parts;
+    rows_shape(n, k, es, &k_part, &parts);
+    const int64_t ldp = up(n, 4);
+    float* part = (float*)sc.take((int64_t)parts * m * ldp * 4);
+    if (!run) return hipSuccess;
+    const bool vec = in_place(a.w, a.ldw, n, es);
+    hipError_t err = with_type(a.dtype, [&](auto* t) {
+      typedef DENSE_T(t) T;
+      if (m == 1) return rows_launch<T, 1>(a, vec, k_part, parts, part, ldp, st);
+      if (m == 2) return rows_launch<T, 2>(a, vec, k_part, parts, part, ldp, st);
+      if (m <= 4) return rows_launch<T, 4>(a, vec, k_part, parts, part, ldp, st);
+      return rows_launch<T, 8>(a, vec, k_part, parts, part, ldp, st);
+    });
+    return err == hipSuccess ? join(a.dtype, part, ldp, parts, m, e, st) : err;
+  }
+  const void *x = a.x, *w = a.w;
+  int64_t ldx = a.ldx, ldw = a.ldw, ka = k, nb = n;
+  if (!in_place(x, ldx, k, es)) {
+    ldx = ka = up(k, 8);
+    void* p = sc.take(m * ldx * es);
+    if (run)
+      if (hipError_t err = pack(a.dtype, x, a.ldx, m, k, p, st)) return err;
+    x = p;
+  }
+  if (!in_place(w, ldw, n, es)) {
+    ldw = nb = up(n, 8);
+    void* p = sc.take(k * ldw * es);
+    if (run)
+      if (hipError_t err = pack(a.dtype, w, a.ldw, k, n, p, st)) return err;
+    w = p;
+  }
+  return product(a.dtype, LAYOUT_NN, x, ldx, w, ldw, m, n, 0, nb, ka, k, e, sc, st, run);
+}
+
+hipError_t backward(const dgprf_linear_grad_t& a, Scratch& sc, hipStream_t st, bool run) {
+  const int es = elem_size(a.dtype);
+  const int64_t m = a.m, k = a.k, n = a.n;
+  hipError_t err = hipSuccess;
+  // dz, unless it is dy and dy can be read in place
+  const bool products = a.dx || a.dw;
+  const bool same = a.act == DGPRF_ACT_NONE && a.drop_thr == 0 && in_place(a.dy, a.lddy, n, es);
+  const void* dz = a.dy;
+  int64_t lddz = a.lddy, na = n;
+  if (products && !same) {
+    lddz = na = up(n, 8);
+    dz = sc.take(m * lddz * es);
+  }
+  if ((products && !same) || a.db) {
+    DzDev d{};
+    d.dy = a.dy;
+    d.aux = a.aux;
+    d.dz = products && !same ? const_cast<void*>(dz) : nullptr;
+    d.lddy = a.lddy;
+    d.ldaux = d.ldz = up(n, 8);
+    d.M = m;
+    d.N = (int)n;
+    d.groups = (int)cdiv(n, 8);
+    d.act = a.act;
+    d.vec = aligned(a.dy, a.lddy, 0, es, 8 * es) ? 1 : 0;
+    d.drop = drop_dev(a.drop_thr, a.seed, a.sub, a.step);
+    const int64_t strips = cdiv(d.groups, 64);
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(cdiv(2048, strips), cdiv(m, 16)));
+    d.rows_part = (int)up(cdiv(m, want), 4);
+    const int64_t parts = cdiv(m, d.rows_part);
+    if (a.db) d.part = (float*)sc.take(parts * d.ldz * 4);
+    if (run) {
+      err = with_type(a.dtype, [&](auto* t) {
+        typedef DENSE_T(t) T;
+        hipLaunchKernelGGL((k_dz<T>), dim3((unsigned)strips, (unsigned)parts), dim3(256), 0, st, d);
+        hipError_t er = hipGetLastError();
+        if (er == hipSuccess && a.db) {
+          hipLaunchKernelGGL((k_db<T>), dim3((unsigned)cdiv(n, 32)), dim3(256), 0, st, d.part, d.ldz, (int)parts,
+                             (int)n, (T*)a.db);
+          er = hipGetLastError();
+        }
+        return er;
+      });
+      if (err != hipSuccess) return err;
+    }
+  }
+  if (a.dx) {  // [m][k] = dz [m][n] (W [k][n])^T
+    const void* w = a.w;
+    int64_t ldw = a.ldw, nb = n;
+    if (!in_place(w, ldw, n, es)) {
+      ldw = nb = up(n, 8);
+      void* p = sc.take(k * ldw * es);
+      if (run && (err = pack(a.dtype, w, a.ldw, k, n, p, st)) != hipSuccess) return err;
+      w = p;
+    }
+    err = product(a.dtype, LAYOUT_NT, dz, lddz, w, ldw, m, k, 0, 0, na, nb, epi_plain(a.dx, k, es), sc, st, run);
+    if (err != hipSuccess) return err;
+  }
+  if (a.dw) {  // [k][n] = (x [m][k])^T dz [m][n]
+    const void* x = a.x;
+    int64_t ldx = a.ldx, ka = k;
+    if (!in_place(x, ldx, k, es)) {
+      ldx = ka = up(k, 8);
+      void* p = sc.take(m * ldx * es);
+      if (run && (err = pack(a.dtype, x, a.ldx, m, k, p, st)) != hipSuccess) return err;
+      x = p;
+    }
+    err = product(a.dtype, LAYOUT_TN, x, ldx, dz, lddz, k, n, ka, na, m, m, epi_plain(a.dw, n, es), sc, st, run);
+  }
+  return err;
+}
+
+// zeros without a memset node (a captured graph replays a fill kernel)
+__global__ __launch_bounds__(256) void k_zero(uint16_t* p, int64_t n) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < n) p[i] = 0;
+}
+hipError_t zero(void* p, int64_t bytes, hipStream_t s) {
+  hipLaunchKernelGGL(k_zero, dim3((unsigned)cdiv(bytes / 2, 256)), dim3(256), 0, s, (uint16_t*)p, bytes / 2);
+  return hipGetLastError();
+}
+
+int hip_rc(hipError_t e) { return e == hipSuccess ? DGPRF_OK : DGPRF_E_HIP; }
+
+int check_forward(const dgprf_linear_t* a) {
+  if (!a) return DGPRF_E_ARG;
+  int rc = check_dims(a->dtype, a->act, a->m, a->k, a->n, a->ldx, a->ldw);
+  if (!rc) rc = check_drop(a->drop_thr);
+  if (!rc && a->res && (a->ldr < 0 || (a->ldr > 0 && a->ldr < a->n))) rc = DGPRF_E_SHAPE;
+  return rc;
+}
+int check_backward(const dgprf_linear_grad_t* a) {
+  if (!a) return DGPRF_E_ARG;
+  int rc = check_dims(a->dtype, a->act, a->m, a->k, a->n, a->ldx, a->ldw);
+  if (!rc) rc = check_drop(a->drop_thr);
+  if (!rc && (a->lddy < 0 || (a->lddy > 0 && a->lddy < a->n) || a->lddy > kMaxWidth)) rc = DGPRF_E_SHAPE;
+  return rc;
+}
+
+}  // namespace
+
+extern "C" {
+
+int dgprf_linear_scratch(const dgprf_linear_t* a, int64_t* bytes_out) {
+  int rc = check_forward(a);
+  if (rc) return rc;
+  if (!bytes_out) return DGPRF_E_ARG;
+  Scratch sc{nullptr};
+  if (a->m > 0) (void)forward(*a, sc, nullptr, false);
+  *bytes_out = sc.used;
+  return DGPRF_OK;
+}
+
+int dgprf_linear_forward(const dgprf_linear_t* a, void* scratch, int64_t scratch_bytes, void* stream) {
+  int64_t need = 0;
+  int rc = dgprf_linear_scratch(a, &need);
+  if (rc) return rc;
+  if (a->m == 0) return DGPRF_OK;
+  if (!a->x || !a->w || !a->y) return DGPRF_E_ARG;
+  if (need > 0 && (!scratch || scratch_bytes < need || (uintptr_t)scratch % 16)) return DGPRF_E_ARG;
+  if (a->aux && (uintptr_t)a->aux % 16) return DGPRF_E_ARG;
+  Scratch sc{(char*)scratch};
+  return hip_rc(forward(*a, sc, reinterpret_cast<hipStream_t>(stream), true));
+}
+
+int dgprf_linear_grad_scratch(const dgprf_linear_grad_t* a, int64_t* bytes_out) {
+  int rc = check_backward(a);
+  if (rc) return rc;
+  if (!bytes_out) return DGPRF_E_ARG;
+  Scratch sc{nullptr};
+  if (a->m > 0) (void)backward(*a, sc, nullptr, false);
+  *bytes_out = sc.used;
+  return DGPRF_OK;
+}
+
+int dgprf_linear_backward(const dgprf_linear_grad_t* a, void* scratch, int64_t scratch_bytes, void* stream) {
+  int64_t need = 0;
+  int rc = dgprf_linear_grad_scratch(a, &need);
+  if (rc) return rc;
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (a->m == 0) {  // sums over no rows
+    const int es = elem_size(a->dtype);
+    hipError_t e = hipSuccess;
+    if (a->dw) e = zero(a->dw, a->k * a->n * es, s);
+    if (e == hipSuccess && a->db) e = zero(a->db, a->n * es, s);
+    return hip_rc(e);
+  }
+  if (!a->dy || (a->dx && !a->w) || (a->dw && !a->x)) return DGPRF_E_ARG;
+  if (a->act != DGPRF_ACT_NONE && !a->aux) return DGPRF_E_ARG;
+  if (a->aux && (uintptr_t)a->aux % 16) return DGPRF_E_ARG;
+  if (need > 0 && (!scratch || scratch_bytes < need || (uintptr_t)scratch % 16)) return DGPRF_E_ARG;
+  Scratch sc{(char*)scratch};
+  return hip_rc(backward(*a, sc, s, true));
+}
+
+int dgprf_dropout(int32_t dtype, const void* x, int64_t rows, int64_t n, int64_t ldx, const void* res,
+                  int64_t ldr, int32_t drop_thr, uint64_t seed, uint64_t sub, const int64_t* step, void* y,
+                  void* stream) {
+  if (dtype != DGPRF_F32 && dtype != DGPRF_F16 && dtype != DGPRF_BF16) return DGPRF_E_ARG;
+  if (check_drop(drop_thr)) return DGPRF_E_ARG;
+  if (rows < 0 || n < 0 || n >= ((int64_t)1 << 31) || (rows > 1 && ldx != 0 && ldx < n) || ldx < 0) return DGPRF_E_SHAPE;
+  if (res && (ldr < 0 || (rows > 1 && ldr != 0 && ldr < n))) return DGPRF_E_SHAPE;
+  if (rows == 0 || n == 0) return DGPRF_OK;
+  if (!x || !y) return DGPRF_E_ARG;
+  const int64_t groups = cdiv(n, 8);
+  if (rows > ((int64_t)1 << 39) / groups) return DGPRF_E_SHAPE;
+  const int es = elem_size(dtype);
+  const int64_t total = rows * groups;
+  const bool flat = n % 8 == 0 && (rows == 1 || ldx == n) && (uintptr_t)x % (8 * es) == 0 &&
+                    (uintptr_t)y % (8 * es) == 0 &&
+                    (!res || ((rows == 1 || ldr == n) && (uintptr_t)res % (8 * es) == 0));
+  const DropDev d = drop_dev(drop_thr, seed, sub, step);
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  return hip_rc(with_type(dtype, [&](auto* t) {
+    typedef DENSE_T(t) T;
+    const dim3 grid((unsigned)cdiv(total, 256));
+    if (flat)
+      hipLaunchKernelGGL((k_dropout<T, true>), grid, dim3(256), 0, s, (const T*)x, ldx, (const T*)res, ldr, (T*)y,
+                         total, (int)groups, (int)n, d);
+    else
+      hipLaunchKernelGGL((k_dropout<T, false>), grid, dim3(256), 0, s, (const T*)x, ldx, (const T*)res, ldr, (T*)y,
+                         total, (int)groups, (int)n, d);
+    return hipGetLastError();
+  }));
+}
+
+}  // extern "C"

@@ -1,0 +1,227 @@
+// dense_common.h — what the kernels of the dense operators share (dense.hip, dense_gemm_impl.h):
+// element types, the activations and their slopes, the dropout mask of the counter-based generator,
+// and the epilogue arguments.
+//
+//   z = x W + b        y = r + s m a(z)        dropout:  y = r + s m x
+//
+// Sums, the bias, the activation, the mask's scale and the residual are in 32 bits; a value is
+// rounded to the tensors' type once, where it is stored.
+#pragma once
+#include <type_traits>
+
+#include "dgprf_internal.h"
+
+namespace dense {
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32v4_t __attribute__((ext_vector_type(4)));
+
+template <class T>
+struct Vec {
+  typedef T v4 __attribute__((ext_vector_type(4)));
+  typedef T v8 __attribute__((ext_vector_type(8)));
+};
+
+inline int elem_size(int dtype) { return dtype == DGPRF_F32 ? 4 : 2; }
+
+// ---------------------------------------------------------------- activations
+// Normal distribution function by its tail: for a = |z|, P(Z < -a) = e^{-a^2 / 2} Q(a) with
+// Q(a) = erfcx(a / sqrt 2) / 2, a smooth, slowly falling function fitted (least squares, reweighted
+// towards the smallest maximal relative error, a in [0, 14]) as t (c0 + c1 t + ...), t = 1 / (1 + ca).
+// The negative side keeps its relative precision (no 1 - erf cancellation) and the exponential is
+// the one the slope needs.  Degree 8: 3.2e-8 (4e-7 as evaluated in 32 bits); degree 5, for the
+// 16-bit types whose rounding is 2^-9 and more: 8.2e-6.
+template <class T>
+__device__ __forceinline__ float tail_q(float a) {
+  if constexpr (sizeof(T) == 4) {
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.35f, a, 1.f));
+    float p = -0.02914646826684475f;
+    p = fmaf(p, t, 0.14397425949573517f);
+    p = fmaf(p, t, -0.2557194232940674f);
+    p = fmaf(p, t, 0.1591798961162567f);
+    p = fmaf(p, t, -0.023113638162612915f);
+    p = fmaf(p, t, 0.10550954192876816f);
+    p = fmaf(p, t, 0.11983250081539154f);
+    p = fmaf(p, t, 0.13986191153526306f);
+    p = fmaf(p, t, 0.13962140679359436f);
+    return p * t;
+  } else {
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3f, a, 1.f));
+    float p = -0.07709866762161255f;
+    p = fmaf(p, t, 0.21604043245315552f);
+    p = fmaf(p, t, -0.016951488330960274f);
+    p = fmaf(p, t, 0.1441979855298996f);
+    p = fmaf(p, t, 0.11374157667160034f);
+    p = fmaf(p, t, 0.12007425725460052f);
+    return p * t;
+  }
+}
+
+__device__ __forceinline__ float exp_of(float x) {  // e^x: v_exp_f32 is 2^x to 1 ulp
+  return __builtin_amdgcn_exp2f(x * 1.4426950408889634f);
+}
+__device__ __forceinline__ float gauss(float z) {  // e^{-z^2 / 2}
+  return __builtin_amdgcn_exp2f(z * z * -0.7213475204444817f);
+}
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + exp_of(-z)); }
+// sqrt(2 / pi) (z + 0.044715 z^3), twice: tanh u = 2 sigmoid(2 u) - 1, so 0.5 z (1 + tanh u) = z sigmoid(2 u)
+__device__ __forceinline__ float tanh_arg2(float z) {
+  return 1.5957691216057308f * z * fmaf(0.044715f, z * z, 1.f);
+}
+
+template <class T, int ACT>
+__device__ __forceinline__ float act_of(float z) {
+  if constexpr (ACT == DGPRF_ACT_RELU) return z < 0.f ? 0.f : z;  // a NaN stays one
+  if constexpr (ACT == DGPRF_ACT_GELU) {
+    const float tail = tail_q<T>(fabsf(z)) * gauss(z);
+    return z * (z < 0.f ? tail : 1.f - tail);
+  }
+  if constexpr (ACT == DGPRF_ACT_GELU_TANH) return z * sigmoid(tanh_arg2(z));
+  if constexpr (ACT == DGPRF_ACT_SILU) return z * sigmoid(z);
+  return z;
+}
+
+// a'(z).  z is clamped in the products that vanish for large |z|, so an infinite z has the limit
+// (0 or 1) and not inf * 0.
+template <class T, int ACT>
+__device__ __forceinline__ float slope_of(float z) {
+  const float zc = __builtin_amdgcn_fmed3f(z, -60.f, 60.f);
+  if constexpr (ACT == DGPRF_ACT_RELU) return z > 0.f ? 1.f : 0.f;
+  if constexpr (ACT == DGPRF_ACT_GELU) {
+    const float e = gauss(z), tail = tail_q<T>(fabsf(z)) * e;
+    return fmaf(zc * 0.3989422804014327f, e, z < 0.f ? tail : 1.f - tail);
+  }
+  if constexpr (ACT == DGPRF_ACT_GELU_TANH) {
+    // g = sigmoid(2u): g + z g (1 - g) 2u'
+    const float g = sigmoid(tanh_arg2(z));
+    return fmaf(zc * g * (1.f - g), 1.5957691216057308f * fmaf(3.f * 0.044715f, zc * zc, 1.f), g);
+  }
+  if constexpr (ACT == DGPRF_ACT_SILU) {
+    const float g = sigmoid(z);
+    return fmaf(zc * g, 1.f - g, g);
+  }
+  return 1.f;
+}
+
+// f(act) with the activation as a compile-time constant
+template <class F>
+__device__ __forceinline__ void with_act(int act, F f) {
+  switch (act) {
+    case DGPRF_ACT_RELU: f(std::integral_constant<int, DGPRF_ACT_RELU>()); break;
+    case DGPRF_ACT_GELU: f(std::integral_constant<int, DGPRF_ACT_GELU>()); break;
+    case DGPRF_ACT_GELU_TANH: f(std::integral_constant<int, DGPRF_ACT_GELU_TANH>()); break;
+    case DGPRF_ACT_SILU: f(std::integral_constant<int, DGPRF_ACT_SILU>()); break;
+    default: f(std::integral_constant<int, DGPRF_ACT_NONE>()); break;
+  }
+}
+
+// What the backward pass needs of z, as it is stored.  Rounding z costs the slope less than the
+// rounding of dz itself costs (z a''(z) is below 0.4); relu's slope is stored instead, because a
+// small z could round to the other side of its jump.
+template <int ACT>
+__device__ __forceinline__ float saved_of(float z) {
+  if constexpr (ACT == DGPRF_ACT_RELU) return z > 0.f ? 1.f : 0.f;
+  return z;
+}
+
+// ---------------------------------------------------------------- dropout mask
+// Eight elements of a row share one Philox4x32-10 call, 16 bits each: p is a multiple of 1 / 65536,
+// and one call costs about what the loads and stores of eight 16-bit elements cost at full
+// bandwidth (32 bits for each would make the generator the bound).  The counter is the group's
+// number, so the mask does not depend on how a kernel is tiled and backward makes it again.
+struct DropDev {
+  uint32_t thr;  // an element is kept when its 16 bits >= thr; 0: no dropout, 65536: drops all
+  float scale;   // 65536 / (65536 - thr); 0 when everything is dropped
+  uint32_t k0, k1;
+  uint64_t sub;
+  const int64_t* step;  // device counter added to sub, or null
+};
+
+__device__ __forceinline__ uint64_t drop_sub(const DropDev& d) {
+  return d.sub + (d.step ? (uint64_t)*d.step : 0ull);
+}
+__device__ __forceinline__ u32x4 drop_words(const DropDev& d, uint64_t sub, uint64_t q) {
+  u32x4 c;
+  c.x = (uint32_t)q;
+  c.y = (uint32_t)sub;
+  c.z = (uint32_t)(sub >> 32);
+  c.w = ((uint32_t)DGPRF_RNG_DROPOUT << 24) | ((uint32_t)(q >> 32) & 0x00FFFFFFu);
+  return philox4x32_10(c, d.k0, d.k1);
+}
+// keep or drop elements 2 i and 2 i + 1 by word i
+__device__ __forceinline__ float drop_lo(float v, uint32_t word, const DropDev& d) {
+  return (word & 0xFFFFu) >= d.thr ? v * d.scale : 0.f;
+}
+__device__ __forceinline__ float drop_hi(float v, uint32_t word, const DropDev& d) {
+  return (word >> 16) >= d.thr ? v * d.scale : 0.f;
+}
+
+// ---------------------------------------------------------------- epilogue
+struct EpiDev {
+  const void* bias;  // [n] or null
+  const void* res;   // [m][ldr] or null
+  void* y;           // [m][ldy]
+  void* aux;         // [m][ldaux] saved z (relu: slope) or null; 16-byte aligned rows
+  int64_t ldr, ldy, ldaux;
+  int32_t n, act;
+  int32_t groups;    // ceil(n / 8)
+  int32_t vec_y, vec_r;  // rows of y / res are aligned for 4 elements at a time
+  DropDev drop;
+};
+
+template <class T>
+__device__ __forceinline__ f4 load4(const T* p) {
+  const typename Vec<T>::v4 v = *reinterpret_cast<const typename Vec<T>::v4*>(p);
+  return __builtin_convertvector(v, f4);
+}
+template <class T>
+__device__ __forceinline__ void store4(T* p, f4 v) {
+  *reinterpret_cast<typename Vec<T>::v4*>(p) = __builtin_convertvector(v, typename Vec<T>::v4);
+}
+// columns col .. col + 3 of a row of n; aligned: the row allows 4-element accesses
+template <class T>
+__device__ __forceinline__ f4 load4_edge(const T* row, int col, int n, bool aligned) {
+  if (aligned && col + 4 <= n) return load4(row + col);
+  f4 v = f4zero();
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    if (col + c < n) v[c] = (float)row[col + c];
+  return v;
+}
+template <class T>
+__device__ __forceinline__ void store4_edge(T* row, int col, int n, bool aligned, f4 v) {
+  if (aligned && col + 4 <= n) {
+    store4(row + col, v);
+    return;
+  }
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    if (col + c < n) row[col + c] = (T)v[c];
+}
+
+// ---------------------------------------------------------------- tiled product
+// C[i][j] = sum_k A(i, k) B(k, j).  "K-contiguous" operands have k innermost in memory (A[i][k],
+// B[j][k]), "K-strided" ones their row or column index (A[k][i], B[k][j]).
+struct GemmArgs {
+  const void *A, *B;
+  int64_t lda, ldb;
+  int32_t I, J;
+  int32_t Ia, Ja;  // K-strided operands: columns that may be read (I, J rounded up where padded)
+  int32_t Ka, Kb;  // K extent of A and B (they differ by A's zero padding)
+  int32_t n_mt, n_nt, splits, stages, stages_split;
+  float* part;     // split-K partials [splits][I][ldp], or null
+  int64_t ldp;
+};
+
+enum { LAYOUT_NN = 0, LAYOUT_NT = 1, LAYOUT_TN = 2 };  // forward, dx, dW
+enum { TILE_256 = 0, TILE_128 = 1, TILE_32 = 2 };
+
+// one instantiation per element type (dense_<type>.hip): layout, tile, and epilogue (part == null:
+// the linear epilogue e; otherwise partial sums)
+hipError_t launch_gemm_bf16(int layout, int tile, const GemmArgs& a, const EpiDev& e, hipStream_t s);
+hipError_t launch_gemm_f16(int layout, int tile, const GemmArgs& a, const EpiDev& e, hipStream_t s);
+hipError_t launch_gemm_f32(int layout, int tile, const GemmArgs& a, const EpiDev& e, hipStream_t s);
+
+}  // namespace dense

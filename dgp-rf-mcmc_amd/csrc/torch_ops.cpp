@@ -12,6 +12,8 @@
 //                          utils.py:10-44, models/regression_model.py:33-50,
 //                          experiments/utils_training.py:63-65
 //   dgprf::lse_finalize    experiments/utils_training.py:79-85
+//   dgprf::linear, linear_backward, dropout   the dense operators (include/dgprf.h): every size,
+//                          type and stride is checked here, before anything is enqueued
 #include <cmath>
 #include <cstring>
 #include <string>
@@ -19,6 +21,7 @@
 
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 
@@ -233,6 +236,155 @@ std::tuple<Tensor, Tensor> lse_finalize(const Tensor& m, const Tensor& s, const 
   return {out, lo};
 }
 
+// ---------------------------------------------------------------- dense operators
+int32_t dense_type(const Tensor& t, const char* what) {
+  TORCH_CHECK(t.is_cuda(), "dgprf: ", what, " must be a HIP tensor");
+  if (t.scalar_type() == at::kFloat) return DGPRF_F32;
+  if (t.scalar_type() == at::kHalf) return DGPRF_F16;
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kBFloat16, "dgprf: ", what,
+                   " must be float32, float16 or bfloat16, got ", t.scalar_type());
+  return DGPRF_BF16;
+}
+// same element type and device as x; [rows, cols] with unit stride within a row
+void dense_like(const Tensor& t, const Tensor& x, int64_t rows, int64_t cols, const char* what) {
+  TORCH_CHECK_TYPE(t.scalar_type() == x.scalar_type(), "dgprf: ", what, " is ", t.scalar_type(), ", x is ",
+                   x.scalar_type(), " (one type for a call)");
+  TORCH_CHECK_VALUE(t.device() == x.device(), "dgprf: ", what, " is on ", t.device(), ", x is on ", x.device());
+  TORCH_CHECK_VALUE(t.dim() == 2 && t.size(0) == rows && t.size(1) == cols, "dgprf: ", what, " must be [", rows,
+                    ", ", cols, "], got ", t.sizes());
+  TORCH_CHECK_VALUE(cols <= 1 || t.stride(1) == 1, "dgprf: ", what, " must have unit stride within a row");
+}
+int64_t row_stride(const Tensor& t) { return t.size(0) <= 1 ? t.size(1) : t.stride(0); }
+
+void check_drop(int64_t thr, const Tensor& x, const OptT& step) {
+  TORCH_CHECK_VALUE(thr >= 0 && thr <= 65536, "dgprf: dropout threshold must be in [0, 65536], got ", thr);
+  if (step.has_value() && step->defined())
+    TORCH_CHECK_VALUE(step->device() == x.device() && step->scalar_type() == at::kLong && step->numel() >= 1,
+                      "dgprf: step must be an int64 tensor on the device of x");
+}
+const int64_t* step_of(const OptT& step) {
+  return step.has_value() && step->defined() ? step->data_ptr<int64_t>() : nullptr;
+}
+const void* ptr_of(const OptT& t) { return t.has_value() && t->defined() ? t->data_ptr() : nullptr; }
+
+// (y [m, n], aux: what backward needs of z, or empty)
+std::tuple<Tensor, Tensor> linear(const Tensor& x, const Tensor& w, const OptT& bias, int64_t act,
+                                  const OptT& res, int64_t thr, int64_t seed, int64_t sub, const OptT& step,
+                                  bool save) {
+  dgprf_linear_t a;
+  std::memset(&a, 0, sizeof(a));
+  a.dtype = dense_type(x, "x");
+  TORCH_CHECK_VALUE(x.dim() == 2 && w.dim() == 2, "dgprf: x and weight must be matrices");
+  a.m = x.size(0);
+  a.k = x.size(1);
+  a.n = w.size(1);
+  dense_like(x, x, a.m, a.k, "x");
+  dense_like(w, x, a.k, a.n, "weight");
+  if (bias.has_value() && bias->defined()) {
+    TORCH_CHECK_VALUE(bias->dim() == 1, "dgprf: bias must be [", a.n, "], got ", bias->sizes());
+    TORCH_CHECK_VALUE(bias->stride(0) == 1 || bias->size(0) <= 1, "dgprf: bias must be contiguous");
+    dense_like(bias->unsqueeze(0), x, 1, a.n, "bias");
+  }
+  if (res.has_value() && res->defined()) {
+    dense_like(*res, x, a.m, a.n, "residual");
+    a.ldr = row_stride(*res);
+  }
+  check_drop(thr, x, step);
+  const c10::DeviceGuard guard(x.device());
+  a.act = (int32_t)act;
+  a.ldx = row_stride(x);
+  a.ldw = row_stride(w);
+  a.x = x.data_ptr();
+  a.w = w.data_ptr();
+  a.bias = ptr_of(bias);
+  a.res = ptr_of(res);
+  a.drop_thr = (int32_t)thr;
+  a.seed = (uint64_t)seed;
+  a.sub = (uint64_t)sub;
+  a.step = step_of(step);
+  int64_t need = 0;
+  check_rc(dgprf_linear_scratch(&a, &need), "dgprf_linear_forward");
+  Tensor y = at::empty({a.m, a.n}, x.options());
+  const bool keep = save && act != DGPRF_ACT_NONE;
+  Tensor aux = at::empty({keep ? a.m : 0, keep ? (a.n + 7) / 8 * 8 : 0}, x.options());
+  a.y = y.data_ptr();
+  a.aux = keep ? aux.data_ptr() : nullptr;
+  Tensor scratch;
+  if (need) scratch = at::empty({need}, x.options().dtype(at::kByte));
+  check_rc(dgprf_linear_forward(&a, need ? scratch.data_ptr() : nullptr, need, stream()),
+           "dgprf_linear_forward");
+  return {y, aux};
+}
+
+// gradients of x, weight and bias (those asked for; the others are empty)
+std::tuple<Tensor, Tensor, Tensor> linear_backward(const Tensor& dy, const Tensor& x, const Tensor& w,
+                                                   const OptT& aux, int64_t act, int64_t thr, int64_t seed,
+                                                   int64_t sub, const OptT& step, bool want_x, bool want_w,
+                                                   bool want_b) {
+  dgprf_linear_grad_t a;
+  std::memset(&a, 0, sizeof(a));
+  a.dtype = dense_type(x, "x");
+  TORCH_CHECK_VALUE(x.dim() == 2 && w.dim() == 2, "dgprf: x and weight must be matrices");
+  a.m = x.size(0);
+  a.k = x.size(1);
+  a.n = w.size(1);
+  dense_like(x, x, a.m, a.k, "x");
+  dense_like(w, x, a.k, a.n, "weight");
+  dense_like(dy, x, a.m, a.n, "dy");
+  if (act != DGPRF_ACT_NONE) {
+    TORCH_CHECK_VALUE(aux.has_value() && aux->defined(), "dgprf: the saved tensor of the forward pass is missing");
+    dense_like(*aux, x, a.m, (a.n + 7) / 8 * 8, "aux");
+    TORCH_CHECK_VALUE(aux->is_contiguous(), "dgprf: aux must be contiguous");
+    a.aux = aux->data_ptr();
+  }
+  check_drop(thr, x, step);
+  const c10::DeviceGuard guard(x.device());
+  a.act = (int32_t)act;
+  a.ldx = row_stride(x);
+  a.ldw = row_stride(w);
+  a.lddy = row_stride(dy);
+  a.x = x.data_ptr();
+  a.w = w.data_ptr();
+  a.dy = dy.data_ptr();
+  a.drop_thr = (int32_t)thr;
+  a.seed = (uint64_t)seed;
+  a.sub = (uint64_t)sub;
+  a.step = step_of(step);
+  const auto none = std::vector<int64_t>{0};
+  Tensor dx = want_x ? at::empty({a.m, a.k}, x.options()) : at::empty(none, x.options());
+  Tensor dw = want_w ? at::empty({a.k, a.n}, x.options()) : at::empty(none, x.options());
+  Tensor db = want_b ? at::empty({a.n}, x.options()) : at::empty(none, x.options());
+  a.dx = want_x ? dx.data_ptr() : nullptr;
+  a.dw = want_w ? dw.data_ptr() : nullptr;
+  a.db = want_b ? db.data_ptr() : nullptr;
+  int64_t need = 0;
+  check_rc(dgprf_linear_grad_scratch(&a, &need), "dgprf_linear_backward");
+  Tensor scratch;
+  if (need) scratch = at::empty({need}, x.options().dtype(at::kByte));
+  check_rc(dgprf_linear_backward(&a, need ? scratch.data_ptr() : nullptr, need, stream()),
+           "dgprf_linear_backward");
+  return {dx, dw, db};
+}
+
+Tensor dropout(const Tensor& x, const OptT& res, int64_t thr, int64_t seed, int64_t sub, const OptT& step) {
+  const int32_t dtype = dense_type(x, "x");
+  TORCH_CHECK_VALUE(x.dim() == 2, "dgprf: x must be [rows, n]");
+  const int64_t rows = x.size(0), n = x.size(1);
+  dense_like(x, x, rows, n, "x");
+  int64_t ldr = 0;
+  if (res.has_value() && res->defined()) {
+    dense_like(*res, x, rows, n, "residual");
+    ldr = row_stride(*res);
+  }
+  check_drop(thr, x, step);
+  const c10::DeviceGuard guard(x.device());
+  Tensor y = at::empty({rows, n}, x.options());
+  check_rc(dgprf_dropout(dtype, x.data_ptr(), rows, n, row_stride(x), ptr_of(res), ldr, (int32_t)thr,
+                         (uint64_t)seed, (uint64_t)sub, step_of(step), y.data_ptr(), stream()),
+           "dgprf_dropout");
+  return y;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(dgprf, m) {
@@ -258,6 +410,11 @@ TORCH_LIBRARY(dgprf, m) {
       "-> ()");
   m.def("lse_finalize(Tensor m, Tensor s, Tensor? e, float s_total, float y_std, bool lse_out) "
         "-> (Tensor, Tensor)");
+  m.def("linear(Tensor x, Tensor weight, Tensor? bias, int act, Tensor? residual, int drop_thr, int seed, "
+        "int sub, Tensor? step, bool save) -> (Tensor, Tensor)");
+  m.def("linear_backward(Tensor dy, Tensor x, Tensor weight, Tensor? aux, int act, int drop_thr, int seed, "
+        "int sub, Tensor? step, bool want_x, bool want_w, bool want_b) -> (Tensor, Tensor, Tensor)");
+  m.def("dropout(Tensor x, Tensor? residual, int drop_thr, int seed, int sub, Tensor? step) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(dgprf, CUDA, m) {
@@ -266,4 +423,7 @@ TORCH_LIBRARY_IMPL(dgprf, CUDA, m) {
   m.impl("forward", &forward);
   m.impl("forward_samples", &forward_samples);
   m.impl("lse_finalize", &lse_finalize);
+  m.impl("linear", &linear);
+  m.impl("linear_backward", &linear_backward);
+  m.impl("dropout", &dropout);
 }

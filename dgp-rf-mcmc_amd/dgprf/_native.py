@@ -20,6 +20,9 @@ BATCH_DIRECT, BATCH_INDEXED, BATCH_EPOCH = 0, 1, 2
 SCHED_CONST, SCHED_CYCLICAL = 0, 1
 RNG_NOISE, RNG_RESAMPLE, RNG_Z, RNG_W, RNG_MOMENTS = 1, 2, 3, 4, 5
 RNG_HYPER, RNG_HYPER_RESAMPLE = 6, 7
+RNG_DROPOUT = 8
+F32, F16, BF16 = 0, 1, 2
+ACTS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 HYP_KERNEL, HYP_LIK, HYP_MEAN = 1, 2, 4
 HMASS = 32  # hmass slots: log_amp l -> l, log_inv_ls l -> 8 + l, mean l -> 16 + l, lik_log_var -> 24
 ABI_VERSION = 10
@@ -80,6 +83,22 @@ class Step(ctypes.Structure):
                 ("xi_resample", _vp), ("xi_hyp", _vp), ("xi_hyp_resample", _vp)]
 
 
+class Linear(ctypes.Structure):
+    """dgprf_linear_t."""
+    _fields_ = [("dtype", _i32), ("act", _i32), ("m", _i64), ("k", _i64), ("n", _i64),
+                ("ldx", _i64), ("ldw", _i64), ("ldr", _i64), ("x", _vp), ("w", _vp),
+                ("bias", _vp), ("res", _vp), ("y", _vp), ("aux", _vp), ("drop_thr", _i32),
+                ("pad0", _i32), ("seed", _u64), ("sub", _u64), ("step", _vp)]
+
+
+class LinearGrad(ctypes.Structure):
+    """dgprf_linear_grad_t."""
+    _fields_ = [("dtype", _i32), ("act", _i32), ("m", _i64), ("k", _i64), ("n", _i64),
+                ("ldx", _i64), ("ldw", _i64), ("lddy", _i64), ("x", _vp), ("w", _vp),
+                ("aux", _vp), ("dy", _vp), ("dx", _vp), ("dw", _vp), ("db", _vp),
+                ("drop_thr", _i32), ("pad0", _i32), ("seed", _u64), ("sub", _u64), ("step", _vp)]
+
+
 # name -> (restype, argtypes); must match include/dgprf.h exactly.
 SIGNATURES = {
     "dgprf_abi_version": (_i32, []),
@@ -117,6 +136,12 @@ SIGNATURES = {
     "dgprf_welford_update": (_i32, [ctypes.POINTER(Plan), _vp, _vp, _vp, _i32, _i32, _vp]),
     "dgprf_mass_estimate": (_i32, [ctypes.POINTER(Plan), _vp, _vp, _i32, _i32, _i32, _vp, _vp,
                                    _vp]),
+    "dgprf_linear_scratch": (_i32, [ctypes.POINTER(Linear), ctypes.POINTER(_i64)]),
+    "dgprf_linear_grad_scratch": (_i32, [ctypes.POINTER(LinearGrad), ctypes.POINTER(_i64)]),
+    "dgprf_linear_forward": (_i32, [ctypes.POINTER(Linear), _vp, _i64, _vp]),
+    "dgprf_linear_backward": (_i32, [ctypes.POINTER(LinearGrad), _vp, _i64, _vp]),
+    "dgprf_dropout": (_i32, [_i32, _vp, _i64, _i64, _i64, _vp, _i64, _i32, _u64, _u64, _vp, _vp,
+                             _vp]),
 }
 
 _lib = None

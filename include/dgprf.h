@@ -56,6 +56,7 @@ extern "C" {
 #define DGPRF_RNG_MOMENTS 5    /* initial momenta                 (models/dgp.py:240) */
 #define DGPRF_RNG_HYPER 6      /* xi of the hyper-parameter updates (full_bayesian=True) */
 #define DGPRF_RNG_HYPER_RESAMPLE 7 /* resampled hyper-parameter momenta          */
+#define DGPRF_RNG_DROPOUT 8    /* dropout masks of dgprf_linear_* / dgprf_dropout */
 
 /* Trainable hyper-parameter groups of full_bayesian=True (plan.hyp_flags; models/dgp.py:175-181,
  * 199-204): the kernels' log_amplitude and log_inv_length_scale (kernel_trainable,
@@ -400,6 +401,88 @@ int dgprf_welford_update(const dgprf_plan_t *plan, const float *grad, float *mea
 int dgprf_mass_estimate(const dgprf_plan_t *plan, const float *mean, const float *m2,
                         int32_t k_batches, int32_t centered, int32_t full_bayes, float *mass_est,
                         float *hmass_est, void *stream);
+
+/* ---------------- dense operators ---------------- */
+/* A dense layer and dropout, forward and backward, for networks around the random-feature layers
+ * (feature extractors, deterministic and MC-dropout baselines).  x W is GPLayer's product
+ * (layers/GP_weight_layers.py:13), W [k][n] in its layout.
+ *
+ *   z = x W + b        y = r + s m a(z)        dropout:  y = r + s m x
+ *
+ * a: DGPRF_ACT_*.  m is 0 for a share thr / 65536 of the elements and 1 for the others, s =
+ * 65536 / (65536 - thr) (thr = 65536 drops everything; a dropped element is 0 whatever its value,
+ * infinities and NaN included).  m is not stored: the elements 8 g .. 8 g + 7 of row i share one
+ * Philox4x32-10 call with key `seed` and counter (q mod 2^32, sub', sub' div 2^32, DGPRF_RNG_DROPOUT
+ * 2^24 + q div 2^32), q = i ceil(n / 8) + g, sub' = sub + (step ? *step : 0); element e of them takes
+ * the half e mod 2 (0: the low one) of word e div 2 and is kept when that half is >= thr.  So the mask
+ * depends on (seed, sub', i, j, n) alone, and backward, given the same, makes it again; a captured
+ * call draws a new mask on each replay when the caller advances *step (between its backward and the
+ * next forward).
+ *
+ * All tensors of a call have one element type (DGPRF_F32 / F16 / BF16) and unit stride within a row.
+ * Sums, bias, activation, mask and residual are in 32 bits; a value is rounded once, where it is
+ * stored.  16-bit backward passes round dz to the type before its two products.
+ * Sizes: k, n and the row strides up to 2^20, m below 2^31; m = 0 is allowed. */
+#define DGPRF_F32 0
+#define DGPRF_F16 1
+#define DGPRF_BF16 2
+
+#define DGPRF_ACT_NONE 0
+#define DGPRF_ACT_RELU 1
+#define DGPRF_ACT_GELU 2       /* z Phi(z) */
+#define DGPRF_ACT_GELU_TANH 3  /* 0.5 z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) */
+#define DGPRF_ACT_SILU 4       /* z / (1 + e^-z) */
+
+typedef struct dgprf_linear {
+  int32_t dtype;
+  int32_t act;
+  int64_t m, k, n;
+  int64_t ldx, ldw, ldr;   /* row strides in elements (ldr = 0: one row for all) */
+  const void *x;           /* [m][k] */
+  const void *w;           /* [k][n] */
+  const void *bias;        /* [n] or NULL */
+  const void *res;         /* [m][n] or NULL */
+  void *y;                 /* [m][n], rows without gaps */
+  void *aux;               /* [m][ceil(n / 8) 8], 16-byte aligned: what backward needs of z, or NULL;
+                              not used for DGPRF_ACT_NONE */
+  int32_t drop_thr;        /* 0 .. 65536 */
+  int32_t pad0;
+  uint64_t seed;
+  uint64_t sub;
+  const int64_t *step;     /* device counter added to sub, or NULL */
+} dgprf_linear_t;
+
+typedef struct dgprf_linear_grad {
+  int32_t dtype;
+  int32_t act;
+  int64_t m, k, n;
+  int64_t ldx, ldw, lddy;  /* lddy = 0: one row for all */
+  const void *x;
+  const void *w;
+  const void *aux;         /* as the forward pass wrote it (NULL for DGPRF_ACT_NONE) */
+  const void *dy;          /* [m][n]: also the residual's gradient */
+  void *dx;                /* [m][k], rows without gaps, or NULL */
+  void *dw;                /* [k][n], or NULL */
+  void *db;                /* [n], or NULL */
+  int32_t drop_thr;
+  int32_t pad0;
+  uint64_t seed;
+  uint64_t sub;
+  const int64_t *step;
+} dgprf_linear_grad_t;
+
+/* Bytes of device scratch (16-byte aligned, owned by the caller, contents of no meaning before or
+ * after) for this call, by its sizes and its pointers' alignment.  Host-only. */
+int dgprf_linear_scratch(const dgprf_linear_t *a, int64_t *bytes_out);
+int dgprf_linear_grad_scratch(const dgprf_linear_grad_t *a, int64_t *bytes_out);
+int dgprf_linear_forward(const dgprf_linear_t *a, void *scratch, int64_t scratch_bytes,
+                         void *stream);
+int dgprf_linear_backward(const dgprf_linear_grad_t *a, void *scratch, int64_t scratch_bytes,
+                          void *stream);
+/* y [rows][n] (rows without gaps) = res + s m x; its backward is the same call on dy without res. */
+int dgprf_dropout(int32_t dtype, const void *x, int64_t rows, int64_t n, int64_t ldx,
+                  const void *res, int64_t ldr, int32_t drop_thr, uint64_t seed, uint64_t sub,
+                  const int64_t *step, void *y, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,104 @@
+"""What the dense operators refuse, and their C structs and scratch sizes: no GPU needed."""
+import ctypes
+import json
+import os
+import subprocess
+
+import pytest
+import torch
+
+import dgprf
+from dgprf import _native as N
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def linear(**kw):
+    a = dict(dtype=N.F32, act=0, m=4, k=8, n=16, ldx=8, ldw=16, ldr=0)
+    a.update(kw)
+    return N.Linear(**a)
+
+
+def grad(**kw):
+    a = dict(dtype=N.F32, act=0, m=4, k=8, n=16, ldx=8, ldw=16, lddy=16)
+    a.update(kw)
+    return N.LinearGrad(**a)
+
+
+def scratch(a):
+    need = ctypes.c_int64(-1)
+    f = N.lib().dgprf_linear_scratch if isinstance(a, N.Linear) else N.lib().dgprf_linear_grad_scratch
+    return f(ctypes.byref(a), ctypes.byref(need)), need.value
+
+
+def test_struct_layout_matches_c(tmp_path):
+    structs = {"dgprf_linear_t": N.Linear, "dgprf_linear_grad_t": N.LinearGrad}
+    lines = ['#include <stdio.h>', '#include <stddef.h>', f'#include "{ROOT}/include/dgprf.h"', 'int main(void){',
+             'printf("{\\"x\\": 0");']
+    for c, cls in structs.items():
+        lines += [f'printf(",\\"{c}.{f}\\": %zu", offsetof({c}, {f}));' for f, _ in cls._fields_]
+        lines.append(f'printf(",\\"{c}\\": %zu", sizeof({c}));')
+    src = tmp_path / "layout.c"
+    src.write_text("\n".join(lines + ['printf("}");', 'return 0;}']))
+    subprocess.check_call(["gcc", "-std=c99", "-o", str(tmp_path / "layout"), str(src)])
+    got = json.loads(subprocess.check_output([str(tmp_path / "layout")]))
+    for c, cls in structs.items():
+        assert got[c] == ctypes.sizeof(cls)
+        assert all(got[f"{c}.{f}"] == getattr(cls, f).offset for f, _ in cls._fields_)
+
+
+@pytest.mark.parametrize("make", [linear, grad])
+@pytest.mark.parametrize("bad", [
+    dict(dtype=3), dict(dtype=-1), dict(act=5), dict(act=-1), dict(drop_thr=-1), dict(drop_thr=65537)])
+def test_arguments_refused(make, bad):
+    assert scratch(make(**bad))[0] == N.E_ARG
+
+
+@pytest.mark.parametrize("make", [linear, grad])
+@pytest.mark.parametrize("bad", [
+    dict(m=-1), dict(k=0), dict(n=0), dict(ldx=7), dict(ldw=15), dict(m=1 << 31), dict(k=(1 << 20) + 1, ldx=(1 << 20) + 1),
+    dict(ldw=(1 << 20) + 1), dict(ldx=(1 << 20) + 1)])
+def test_shapes_refused(make, bad):
+    assert scratch(make(**bad))[0] == N.E_SHAPE
+
+
+def test_calls_refused_before_anything_is_enqueued():
+    lib, e = N.lib(), ctypes.byref
+    assert lib.dgprf_linear_forward(None, None, 0, None) == N.E_ARG
+    assert lib.dgprf_linear_backward(None, None, 0, None) == N.E_ARG
+    assert lib.dgprf_linear_scratch(e(linear()), None) == N.E_ARG
+    assert lib.dgprf_linear_forward(e(linear()), None, 0, None) == N.E_ARG      # no tensors
+    some = 1 << 20  # never read: refused on the host
+    ok = dict(x=some, w=some, y=some)
+    assert scratch(linear(**ok))[1] > 0
+    assert lib.dgprf_linear_forward(e(linear(**ok)), None, 0, None) == N.E_ARG   # scratch missing
+    assert lib.dgprf_linear_forward(e(linear(**ok)), some, 1, None) == N.E_ARG   # scratch too small
+    assert lib.dgprf_linear_forward(e(linear(res=some, ldr=3, **ok)), some, 1 << 30, None) == N.E_SHAPE
+    assert lib.dgprf_linear_forward(e(linear(act=2, aux=some + 4, **ok)), some, 1 << 30, None) == N.E_ARG
+    g = dict(x=some, w=some, dy=some, dx=some)
+    assert lib.dgprf_linear_backward(e(grad(act=2, **g)), some, 1 << 30, None) == N.E_ARG  # nothing saved
+    assert lib.dgprf_linear_backward(e(grad(lddy=3, **g)), some, 1 << 30, None) == N.E_SHAPE
+    assert lib.dgprf_dropout(9, some, 1, 8, 8, None, 0, 0, 0, 0, None, some, None) == N.E_ARG
+    assert lib.dgprf_dropout(0, some, 1, 8, 8, None, 0, 65537, 0, 0, None, some, None) == N.E_ARG
+    assert lib.dgprf_dropout(0, some, 2, 8, 4, None, 0, 1, 0, 0, None, some, None) == N.E_SHAPE
+    assert lib.dgprf_dropout(0, some, -1, 8, 8, None, 0, 1, 0, 0, None, some, None) == N.E_SHAPE
+    assert lib.dgprf_dropout(0, None, 1, 8, 8, None, 0, 1, 0, 0, None, None, None) == N.E_ARG
+    # nothing to do
+    assert lib.dgprf_linear_forward(e(linear(m=0)), None, 0, None) == 0
+    assert lib.dgprf_dropout(0, None, 0, 8, 8, None, 0, 1, 0, 0, None, None, None) == 0
+
+
+def test_python_refusals():
+    x, w = torch.zeros(4, 8), torch.zeros(8, 16)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        dgprf.linear(x, w)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        dgprf.dropout(x, 0.5)
+    with pytest.raises(TypeError):
+        dgprf.linear(x.double(), w)
+    with pytest.raises(TypeError):
+        dgprf.linear([[1.0]], w)
+    for p in (-0.1, 1.1, float("nan")):
+        with pytest.raises(ValueError):
+            dgprf.dense.drop_threshold(p)
+    assert [dgprf.dense.drop_threshold(p) for p in (0, 0.1, 0.5, 1)] == [0, 6554, 32768, 65536]

@@ -1,0 +1,402 @@
+"""The dense operators (dgprf.linear, dgprf.dropout) against their definition in float64: sizes from
+one row to many tiles, odd sizes, strides, masks, every type and activation, gradients, streams and
+captured graphs."""
+import numpy as np
+import pytest
+import torch
+
+import dgprf
+from dgprf import _native as N
+from dense_reference import ACTS, TYPES, Linear, check, keep_mask, scale_of
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _gen(seed):
+    g = torch.Generator()
+    g.manual_seed(seed)
+    return g
+
+
+def normal(g, *shape, t=torch.float32, scale=1.0):
+    return (torch.randn(*shape, generator=g) * scale).to(t)
+
+
+def grid(g, *shape, t=torch.float32, top=2):
+    """Small whole numbers: their products and sums are exact in 32 bits, in any order."""
+    return torch.randint(-top, top + 1, shape, generator=g).to(t)
+
+
+def run(x, w, b=None, act="none", r=None, p=0.0, seed=0, sub=0, dy=None, **kw):
+    """Result and gradients of CPU arguments, on the GPU."""
+    leaf = [None if v is None else v.to(DEV).requires_grad_(dy is not None) for v in (x, w, b, r)]
+    y = dgprf.linear(leaf[0], leaf[1], leaf[2], act, leaf[3], p, seed, sub, **kw)
+    if dy is None:
+        return (y,)
+    asked = [v for v in leaf if v is not None]
+    got = iter(torch.autograd.grad(y, asked, dy.to(DEV)))
+    return (y, *(None if v is None else next(got) for v in leaf))
+
+
+# rows of the streaming kernel (1 .. 8), of the 32-row tile, of 128- and 256-wide tiles; K and N below, at
+# and above a 16-byte piece, a fragment, a stage and a tile; one and many parts of K
+SIZES = [(1, 1, 1), (1, 64, 64), (1, 2048, 512), (2, 37, 131), (3, 1030, 200), (5, 8, 4096), (8, 1500, 129),
+         (9, 1, 7), (9, 64, 128), (17, 515, 33), (32, 4096, 256), (33, 33, 65), (64, 128, 8), (100, 200, 300),
+         (128, 64, 128), (129, 1025, 257), (255, 72, 1001), (256, 2048, 256), (700, 9, 700), (1000, 333, 5)]
+BIG = [(4096, 72, 2560), (2561, 40, 4097), (4100, 136, 2600)]
+
+
+@pytest.mark.parametrize("tname", TYPES)
+@pytest.mark.parametrize("size", SIZES + BIG, ids=str)
+def test_products_exact(size, tname):
+    """Whole numbers: the sums have no rounding, so results and gradients are the exact ones, rounded
+    to the type once."""
+    m, k, n = size
+    t, g = TYPES[tname], _gen(m * 7 + k * 3 + n)
+    x, w, b, r, dy = grid(g, m, k, t=t), grid(g, k, n, t=t), grid(g, n, t=t), grid(g, m, n, t=t), grid(g, m, n, t=t)
+    if m * k * n > 1e8:  # the reference of the large ones in float32 on the GPU is exact, too
+        d = lambda v: v.to(DEV).float()  # noqa: E731
+    else:
+        d = lambda v: v.double()  # noqa: E731
+    y, dx, dw, db, dr = run(x, w, b, r=r, dy=dy)
+    for name, got, want in (("y", y, d(x) @ d(w) + d(b) + d(r)), ("dx", dx, d(dy) @ d(w).t().contiguous()),
+                            ("dw", dw, d(x).t().contiguous() @ d(dy)), ("db", db, d(dy).sum(0)), ("dr", dr, d(dy))):
+        assert got.dtype == t and torch.equal(got.cpu(), want.to(t).cpu()), name
+
+
+@pytest.mark.parametrize("tname", TYPES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("size", [(1, 300, 200), (6, 65, 77), (40, 256, 136), (200, 784, 300), (130, 515, 261)], ids=str)
+def test_linear_and_gradients(size, act, tname):
+    m, k, n = size
+    t, g = TYPES[tname], _gen(m + k + n)
+    make = grid if act == "relu" else normal  # relu's slope jumps at 0: z without rounding
+    x, w = make(g, m, k, t=t), make(g, k, n, t=t) if act == "relu" else normal(g, k, n, t=t, scale=k ** -0.5)
+    b, r, dy = make(g, n, t=t), normal(g, m, n, t=t), normal(g, m, n, t=t)
+    p, seed, sub = 0.3, 0x1234567890ABCDEF, (1 << 33) + 5
+    thr = int(p * 65536 + 0.5)
+    ref = Linear(x, w, b, act, r, thr, seed, sub, dy)
+    y, dx, dw, db, dr = run(x, w, b, act, r, p, seed, sub, dy)
+    check(y, ref.y, ref.y_tol, "y")
+    check(dx, ref.dx, ref.dx_tol, "dx")
+    check(dw, ref.dw, ref.dw_tol, "dw")
+    check(db, ref.db, ref.db_tol, "db")
+    assert torch.equal(dr.cpu(), dy)
+    again = run(x, w, b, act, r, p, seed, sub, dy)
+    assert all(torch.equal(u, v) for u, v in zip((y, dx, dw, db), again)), "not the same twice"
+    # without gradients: the same kernel without what backward needs
+    assert torch.equal(run(x, w, b, act, r, p, seed, sub)[0], y)
+    ref = Linear(x, w, None, act)
+    check(run(x, w, None, act)[0], ref.y, ref.y_tol, "y without bias, dropout, residual")
+
+
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+def test_gradient_against_differences(act):
+    """d/dh of sum(dy y) along a direction of x, w and b, by the central difference of the float64
+    definition at h = 2^-10 (third derivatives below 4: off by less than 4 h^2 sum|dy| |dz|^3 / 6)."""
+    g = _gen(3)
+    m, k, n, h = 12, 24, 40, 2.0 ** -10
+    x, w, b, dy = normal(g, m, k), normal(g, k, n, scale=k ** -0.5), normal(g, n, scale=0.1), normal(g, m, n)
+    vx, vw, vb = normal(g, m, k, scale=0.1), normal(g, k, n, scale=0.1 * k ** -0.5), normal(g, n, scale=0.1)
+    thr, seed, sub = 16384, 99, 7
+    from dense_reference import act as f
+    keep = keep_mask(m, n, thr, seed, sub).double() * scale_of(thr)
+
+    def loss(e):
+        z = (x.double() + e * vx.double()) @ (w.double() + e * vw.double()) + b.double() + e * vb.double()
+        return float((dy.double() * keep * f(z, act)).sum())
+
+    want = (loss(h) - loss(-h)) / (2 * h)
+    _, dx, dw, db, _ = run(x, w, b, act, None, 0.25, seed, sub, dy)
+    got = sum(float((d.double().cpu() * v.double()).sum()) for d, v in ((dx, vx), (dw, vw), (db, vb)))
+    ref = Linear(x, w, b, act, None, thr, seed, sub, dy)
+    tol = sum(float((e * v.double().abs()).sum()) for e, v in ((ref.dx_tol, vx), (ref.dw_tol, vw), (ref.db_tol, vb)))
+    dz = vx.double() @ w.double() + x.double() @ vw.double() + vb.double()
+    tol += float(4 * h * h / 6 * (dy.double().abs() * keep * (dz.abs() + 0.1) ** 3).sum()) * 4
+    assert abs(got - want) < tol, (got, want, tol)
+
+
+@pytest.mark.parametrize("tname", TYPES)
+@pytest.mark.parametrize("shape", [(1, 1), (3, 7), (1, 1024), (5, 24), (200, 1024), (17, 1001), (4, 3, 40), (9,)], ids=str)
+@pytest.mark.parametrize("p", [0.0, 0.1, 0.5, 1.0])
+def test_dropout(shape, p, tname):
+    t, g = TYPES[tname], _gen(len(shape) * 100 + shape[-1])
+    x, r, dy = normal(g, *shape, t=t), normal(g, *shape, t=t), normal(g, *shape, t=t)
+    seed, sub, n = 2 ** 63 + 12345, 2 ** 40 + 3, shape[-1]
+    thr = int(p * 65536 + 0.5)
+    keep = keep_mask(x.numel() // n, n, thr, seed, sub).reshape(shape).double()
+    s = np.float32(65536.0 / (65536 - thr)) if thr < 65536 else np.float32(0)
+    # in 32 bits: one product, one sum, one rounding to the type
+    drop = lambda v: torch.where(keep > 0, v.float() * float(s), torch.zeros(()))  # noqa: E731
+    xd, rd = x.to(DEV).requires_grad_(), r.to(DEV).requires_grad_()
+    y = dgprf.dropout(xd, p, residual=rd, seed=seed, sub=sub)
+    dx, dr = torch.autograd.grad(y, (xd, rd), dy.to(DEV))
+    # v_mul then v_add, or one fma: half a step of 32 bits apart, which may change the type's rounding
+    want = drop(x) + r.float()
+    tol = torch.finfo(t).eps / 2 * want.abs().double() + 2.0 ** -23 * (want.abs() + drop(x).abs()).double() + 1e-30
+    if t == torch.float16:
+        tol = tol + 2.0 ** -25
+    check(y, want.double(), tol, "y")
+    assert torch.equal(dx.cpu(), drop(dy).to(t)) and torch.equal(dr.cpu(), dy)
+    assert torch.equal(dgprf.dropout(x.to(DEV), p, seed=seed, sub=sub).cpu(), drop(x).to(t))
+
+
+def test_linear_takes_dropouts_mask():
+    """The mask depends on (seed, sub, row, column, n) alone: every path of linear has the one of dropout."""
+    for m, n in ((1, 40), (7, 136), (20, 264), (150, 100), (513, 130), (4096, 2560)):
+        one, w, b = torch.ones(m, 8, device=DEV), torch.zeros(8, n, device=DEV), torch.ones(n, device=DEV)
+        want = dgprf.dropout(torch.ones(m, n, device=DEV), 0.4, seed=5, sub=6)
+        assert torch.equal(dgprf.linear(one, w, b, dropout=0.4, seed=5, sub=6), want), (m, n)
+        assert 0 < int((want == 0).sum()) < m * n
+        assert not torch.equal(dgprf.linear(one, w, b, dropout=0.4, seed=5, sub=7), want)
+
+
+def test_dropped_elements_are_zero_whatever_they_hold():
+    x = torch.full((64, 256), float("nan"), device=DEV)
+    x[::2] = float("inf")
+    keep = keep_mask(64, 256, 32768, 1, 2).to(DEV)
+    y = dgprf.dropout(x, 0.5, seed=1, sub=2)
+    assert bool((y[~keep] == 0).all()) and not bool(torch.isfinite(y[keep]).any())
+    assert bool((dgprf.dropout(x, 1.0, seed=1, sub=2) == 0).all())
+    # a gradient that is not finite where the mask dropped does not get through
+    v = torch.ones(64, 32, device=DEV, requires_grad=True)
+    w = torch.ones(32, 256, device=DEV, requires_grad=True)
+    y = dgprf.linear(v, w, activation="gelu", dropout=0.5, seed=1, sub=2)
+    dy = torch.where(keep, torch.ones_like(y), torch.full_like(y, float("nan")))
+    assert all(bool(torch.isfinite(d).all()) for d in torch.autograd.grad(y, (v, w), dy))
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("tname", TYPES)
+def test_not_finite_values(tname, act):
+    """An infinite or NaN input reaches its own row of the result and no other; slopes at infinity are
+    the limits 0 or 1."""
+    t, g = TYPES[tname], _gen(1)
+    for m in (4, 70):
+        x, w = normal(g, m, 64, t=t).abs() + 0.5, normal(g, 64, 96, t=t).abs() + 0.5
+        x, w = x.to(DEV), w.to(DEV)
+        clean = dgprf.linear(x, w, activation=act)
+        for bad in (float("inf"), float("nan")):
+            x2 = x.clone()
+            x2[2, 5] = bad
+            x2.requires_grad_()
+            y = dgprf.linear(x2, w, activation=act)
+            assert torch.equal(y[torch.arange(m) != 2], clean[torch.arange(m) != 2])
+            assert bool((torch.isinf(y[2]) if bad == float("inf") else torch.isnan(y[2])).all())
+            dx, = torch.autograd.grad(y, x2, torch.ones_like(y))
+            if bad == float("inf"):
+                assert bool(torch.isfinite(dx).all())
+            else:
+                assert bool(torch.isfinite(dx[torch.arange(m) != 2]).all())
+
+
+@pytest.mark.parametrize("tname", TYPES)
+@pytest.mark.parametrize("m", [3, 24, 150])
+def test_strides(m, tname):
+    """Rows apart, columns of a larger tensor, transposed operands, a residual row for all, odd
+    offsets: the same results as of contiguous copies, and nothing outside is touched."""
+    t, g, k, n = TYPES[tname], _gen(m), 72, 104
+    base = grid(g, m, k + 24, t=t).to(DEV)
+    wide = grid(g, k + 2, n + 8, t=t).to(DEV)
+    bias = grid(g, n, t=t).to(DEV)
+    row = grid(g, 1, n, t=t).to(DEV)
+    dy = grid(g, m, n, t=t).to(DEV)
+
+    def both(x, w, r, dy):
+        out = []
+        for c in (False, True):
+            leaf = [(v.contiguous() if c else v).detach() for v in (x, w, r)]
+            leaf[2] = leaf[2].clone() if c else leaf[2]
+            for v in leaf:
+                v.requires_grad_()
+            y = dgprf.linear(leaf[0], leaf[1], bias, "none", leaf[2])
+            out.append((y, *torch.autograd.grad(y, leaf, dy.contiguous() if c else dy)))
+        for u, v in zip(*out):
+            assert torch.equal(u, v)
+
+    for off in (0, 1, 8):
+        both(base[:, off:off + k], wide[1:k + 1, off:off + n], row.expand(m, n), dy)
+    both(base[:, :k], wide[:k, :n], dy, row.expand(m, n))
+    xt, wt = grid(g, k, m, t=t).to(DEV).t(), grid(g, n, k, t=t).to(DEV).t()
+    both(xt, wt, grid(g, n, m, t=t).to(DEV).t(), grid(g, n, m, t=t).to(DEV).t())
+    both(base[::2, :k], wide[:k, :n], dy[::2], dy[::2])
+    both(base[:, 3:3 + k], wide[:k, 5:5 + n], dy, dy)
+
+
+def test_leading_dimensions_and_no_rows():
+    g = _gen(4)
+    x, w = normal(g, 3, 5, 16).to(DEV).requires_grad_(), normal(g, 16, 24).to(DEV).requires_grad_()
+    b = normal(g, 24).to(DEV).requires_grad_()
+    y = dgprf.linear(x, w, b, "silu")
+    assert y.shape == (3, 5, 24)
+    dx, dw = torch.autograd.grad(y, (x, w), torch.ones_like(y))
+    flat = x.detach().reshape(15, 16).requires_grad_()
+    y2 = dgprf.linear(flat, w, b, "silu")
+    dx2, dw2 = torch.autograd.grad(y2, (flat, w), torch.ones_like(y2))
+    assert torch.equal(y.reshape(15, 24), y2) and torch.equal(dx.reshape(15, 16), dx2) and torch.equal(dw, dw2)
+    v = x[0, 0].detach()
+    assert torch.equal(dgprf.linear(v, w.detach(), b.detach(), "silu"), y2[0].detach()) or \
+        torch.allclose(dgprf.linear(v, w.detach(), b.detach(), "silu"), y2[0].detach(), rtol=1e-5, atol=1e-5)
+    for t in TYPES.values():
+        x0 = torch.empty(0, 16, device=DEV, dtype=t, requires_grad=True)
+        w0, b0 = w.detach().to(t).requires_grad_(), b.detach().to(t).requires_grad_()
+        y0 = dgprf.linear(x0, w0, b0, "gelu", dropout=0.5)
+        assert y0.shape == (0, 24)
+        dx0, dw0, db0 = torch.autograd.grad(y0, (x0, w0, b0), torch.empty_like(y0))
+        assert dx0.shape == (0, 16) and not dw0.any() and not db0.any()
+        assert dgprf.dropout(torch.empty(3, 0, device=DEV, dtype=t), 0.5).shape == (3, 0)
+
+
+def test_gradients_asked_for_alone():
+    g = _gen(5)
+    x, w, b, r = normal(g, 40, 24), normal(g, 24, 56), normal(g, 56), normal(g, 40, 56)
+    dy = normal(g, 40, 56).to(DEV)
+    full = run(x, w, b, "gelu", r, 0.2, 3, 4, dy.cpu())
+    for i in range(4):
+        leaf = [v.to(DEV) for v in (x, w, b, r)]
+        leaf[i].requires_grad_()
+        y = dgprf.linear(*leaf[:3], "gelu", leaf[3], 0.2, 3, 4)
+        got, = torch.autograd.grad(y, leaf[i], dy)
+        assert torch.equal(got, full[1 + i])
+    # one tensor in two places: the sum of its gradients
+    s = normal(g, 24, 24).to(DEV).requires_grad_()
+    y = dgprf.linear(s, s, residual=s)
+    d = torch.ones_like(y)
+    got, = torch.autograd.grad(y, s, d)
+    c = s.detach().double()
+    want = d.double() @ c.t() + c.t() @ d.double() + d.double()
+    assert (got.double() - want).abs().max() < 60 * 2.0 ** -23 * (1 + 2 * c.abs().sum(0).max() + 2 * c.abs().sum(1).max())
+    with pytest.raises(RuntimeError):
+        y = dgprf.linear(s, s, activation="gelu")
+        first, = torch.autograd.grad(y.sum(), s, create_graph=True)
+        torch.autograd.grad(first.sum(), s)
+
+
+def test_masks_come_from_the_global_generator():
+    x = torch.ones(64, 64, device=DEV)
+    dgprf.set_seed(11)
+    a, b = dgprf.dropout(x, 0.5), dgprf.dropout(x, 0.5)
+    assert not torch.equal(a, b)
+    dgprf.set_seed(11)
+    assert torch.equal(a, dgprf.dropout(x, 0.5)) and torch.equal(b, dgprf.dropout(x, 0.5))
+    step = torch.tensor([5], device=DEV)
+    assert torch.equal(dgprf.dropout(x, 0.5, seed=1, sub=2, step=step), dgprf.dropout(x, 0.5, seed=1, sub=7))
+
+
+def _block(x, w1, b1, w2, b2, step=None):
+    """The operators as a network uses them: up-projection, dropout, down-projection onto the residual."""
+    h = dgprf.linear(x, w1, b1, "gelu", dropout=0.2, seed=8, sub=0, step=step)
+    y = dgprf.linear(h, w2, b2, residual=x, dropout=0.1, seed=8, sub=1 << 32, step=step)
+    return dgprf.dropout(y, 0.1, seed=8, sub=1 << 33, step=step)
+
+
+@pytest.mark.parametrize("tname", TYPES)
+def test_block(tname):
+    """A run of the operators against the same in float64 where every operator's result is rounded to
+    the type, as it is when handed on: an error of half a step goes through each later operator."""
+    t, g = TYPES[tname], _gen(6)
+    m, d, f = 96, 64, 200
+    x, w1, b1 = normal(g, m, d, t=t), normal(g, d, f, t=t, scale=d ** -0.5), normal(g, f, t=t, scale=0.1)
+    w2, b2, dy = normal(g, f, d, t=t, scale=f ** -0.5), normal(g, d, t=t, scale=0.1), normal(g, m, d, t=t)
+    leaf = [v.to(DEV).requires_grad_() for v in (x, w1, b1, w2, b2)]
+    y = _block(*leaf)
+    got = torch.autograd.grad(y, leaf, dy.to(DEV))
+    # operator by operator, on what the one before gave
+    h = dgprf.linear(*leaf[:3], "gelu", dropout=0.2, seed=8, sub=0).detach().cpu()
+    r1 = Linear(x, w1, b1, "gelu", None, int(0.2 * 65536 + 0.5), 8, 0)
+    check(h, r1.y, r1.y_tol, "h")
+    thr = int(0.1 * 65536 + 0.5)
+    dy2 = dgprf.dropout(dy.to(DEV), 0.1, seed=8, sub=1 << 33).cpu()
+    r2 = Linear(h, w2, b2, "none", x, thr, 8, 1 << 32, dy2)
+    y2 = dgprf.linear(h.to(DEV), leaf[3].detach(), leaf[4].detach(), residual=leaf[0].detach(), dropout=0.1,
+                      seed=8, sub=1 << 32)
+    check(y2, r2.y, r2.y_tol, "y before the last dropout")
+    assert torch.equal(y, dgprf.dropout(y2, 0.1, seed=8, sub=1 << 33))
+    check(got[3], r2.dw, r2.dw_tol, "dw2")
+    check(got[4], r2.db, r2.db_tol, "db2")
+    hl = h.to(DEV).requires_grad_()
+    dh, = torch.autograd.grad(dgprf.linear(hl, leaf[3], leaf[4], dropout=0.1, seed=8, sub=1 << 32), hl, dy2.to(DEV))
+    r3 = Linear(x, w1, b1, "gelu", None, int(0.2 * 65536 + 0.5), 8, 0, dh.cpu())
+    check(got[1], r3.dw, r3.dw_tol, "dw1")
+    check(got[2], r3.db, r3.db_tol, "db1")
+    eps = torch.finfo(t).eps
+    check(got[0], r3.dx + dy2.double(), r3.dx_tol + eps * (r3.dx.abs() + dy2.double().abs()), "dx")
+
+
+def test_captured_training_step():
+    """Forward and backward captured once and replayed, with eager work between the replays: the
+    device counter gives every replay the mask of the eager call with that number."""
+    g = _gen(7)
+    leaf = [v.to(DEV).requires_grad_() for v in (normal(g, 300, 64), normal(g, 64, 96, scale=0.1), normal(g, 96),
+                                                 normal(g, 96, 64, scale=0.1), normal(g, 64))]
+    dy = normal(g, 300, 64).to(DEV)
+    step = torch.zeros(1, dtype=torch.int64, device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        y = _block(*leaf, step=step)
+        torch.autograd.grad(y, leaf, dy)
+    torch.cuda.current_stream().wait_stream(side)
+    del y
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = _block(*leaf, step=step)
+        got = torch.autograd.grad(y, leaf, dy)
+        step += 1
+    step.zero_()
+    for i in range(4):
+        at = torch.full((1,), i, dtype=torch.int64, device=DEV)
+        y2 = _block(*leaf, step=at)
+        want = torch.autograd.grad(y2, leaf, dy)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, y2) and all(torch.equal(u, v) for u, v in zip(got, want)), i
+        assert int(step) == i + 1
+
+
+def test_two_graphs_and_streams():
+    """Two captured calls do not share scratch, and a call on another stream is ordered there."""
+    g = _gen(8)
+    xs = [normal(g, 20, 2048).to(DEV) for _ in range(2)]
+    w = normal(g, 2048, 512, scale=0.02).to(DEV)
+    want = [dgprf.linear(x, w, activation="gelu") for x in xs]
+    graphs, outs = [], []
+    for x in xs:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(dgprf.linear(x, w, activation="gelu"))
+        graphs.append(gr)
+    for _ in range(3):
+        streams = [torch.cuda.Stream() for _ in graphs]
+        for s, gr in zip(streams, graphs):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                gr.replay()
+        for s in streams:
+            torch.cuda.current_stream().wait_stream(s)
+        torch.cuda.synchronize()
+        assert all(torch.equal(u, v) for u, v in zip(outs, want))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        y = dgprf.linear(xs[0], w, activation="gelu")
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(y, want[0])
+
+
+def test_rows_around_are_left_alone():
+    """The C entry points write the m rows of y and nothing behind them."""
+    import ctypes
+    m, k, n = 21, 40, 30
+    x, w = torch.ones(m, k, device=DEV), torch.ones(k, n, device=DEV)
+    y = torch.full((m + 2, n), 7.0, device=DEV)
+    a = N.Linear(dtype=N.F32, act=0, m=m, k=k, n=n, ldx=k, ldw=n, ldr=0, x=x.data_ptr(), w=w.data_ptr(),
+                 y=y.data_ptr())
+    need = ctypes.c_int64()
+    N.call("dgprf_linear_scratch", ctypes.byref(a), ctypes.byref(need))
+    scratch = torch.empty(max(16, need.value), dtype=torch.uint8, device=DEV)
+    N.call("dgprf_linear_forward", ctypes.byref(a), ctypes.c_void_p(scratch.data_ptr()), need.value,
+           ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    assert bool((y[:m] == k).all()) and bool((y[m:] == 7).all())
