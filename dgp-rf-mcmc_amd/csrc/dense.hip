@@ -30,98 +30,51 @@ __global__ __launch_bounds__(256) void k_pack(const T* __restrict__ in, int64_t 
   *reinterpret_cast<typename Vec<T>::v8*>(out + row * ldo + col) = v;
 }
 
-// ---------------------------------------------------------------- eight columns of a row
-struct F8 {
-  f4 lo, hi;
-};
-template <class T>
-__device__ __forceinline__ F8 load8(const T* row, int col, int n, bool aligned) {
-  F8 v;
-  if (aligned && col + 8 <= n) {
-    const typename Vec<T>::v8 x = *reinterpret_cast<const typename Vec<T>::v8*>(row + col);
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      v.lo[c] = (float)x[c];
-      v.hi[c] = (float)x[c + 4];
-    }
-  } else {
-    v.lo = load4_edge(row, col, n, false);
-    v.hi = load4_edge(row, col + 4, n, false);
-  }
-  return v;
-}
-template <class T>
-__device__ __forceinline__ void store8(T* row, int col, int n, bool aligned, F8 v) {
-  if (aligned && col + 8 <= n) {
-    typename Vec<T>::v8 x;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      x[c] = (T)v.lo[c];
-      x[c + 4] = (T)v.hi[c];
-    }
-    *reinterpret_cast<typename Vec<T>::v8*>(row + col) = x;
-  } else {
-    store4_edge(row, col, n, false, v.lo);
-    store4_edge(row, col + 4, n, false, v.hi);
-  }
-}
-__device__ __forceinline__ F8 drop8(F8 v, const u32x4& w, const DropDev& d) {
-  v.lo[0] = drop_lo(v.lo[0], w.x, d);
-  v.lo[1] = drop_hi(v.lo[1], w.x, d);
-  v.lo[2] = drop_lo(v.lo[2], w.y, d);
-  v.lo[3] = drop_hi(v.lo[3], w.y, d);
-  v.hi[0] = drop_lo(v.hi[0], w.z, d);
-  v.hi[1] = drop_hi(v.hi[1], w.z, d);
-  v.hi[2] = drop_lo(v.hi[2], w.w, d);
-  v.hi[3] = drop_hi(v.hi[3], w.w, d);
-  return v;
-}
-
 // ---------------------------------------------------------------- joining the parts of K
-// Sums the parts in order (so a result does not depend on which part was ready first) and applies the
-// epilogue; one thread for eight columns of a row.  e.y 8-aligned rows: vec.
+// Sums the parts and applies the epilogue.  A workgroup takes 64 groups of eight columns of a row;
+// wave w adds parts w, w + 4, ... (four loads in flight: with few rows the time is the latency of a
+// thread's chain of loads), then the four sums are added in order, so a result does not depend on
+// which part was ready first.
 template <class T>
 __global__ __launch_bounds__(256) void k_join(const float* __restrict__ part, int64_t ldp, int parts,
                                               int64_t rows, const EpiDev e) {
-  const int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (q >= rows * e.groups) return;
-  const int64_t row = q / e.groups;
-  const int col = (int)(q - row * e.groups) * 8, n = e.n;
-  const float* p = part + row * ldp + col;
+  __shared__ __attribute__((aligned(16))) f4 sums[3][2][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t q = (int64_t)blockIdx.x * 64 + lane;
+  const bool live = q < rows * e.groups;
+  const int64_t row = live ? q / e.groups : 0;
+  const int col = live ? (int)(q - row * e.groups) * 8 : 0, n = e.n;
   const int64_t stride = rows * ldp;
-  F8 v;
-  v.lo = f4zero();
-  v.hi = f4zero();
-  const bool hi = col + 4 < ldp;  // ldp % 4 == 0
-  for (int s = 0; s < parts; ++s, p += stride) {
-    v.lo += *reinterpret_cast<const f4*>(p);
-    if (hi) v.hi += *reinterpret_cast<const f4*>(p + 4);
+  F8 v{f4zero(), f4zero()};
+  if (live) {
+    const float* p = part + row * ldp + col;  // ldp % 8 == 0
+#pragma unroll 4
+    for (int s = wave; s < parts; s += 4) {
+      v.lo += *reinterpret_cast<const f4*>(p + s * stride);
+      v.hi += *reinterpret_cast<const f4*>(p + s * stride + 4);
+    }
   }
-  if (e.bias) {
-    v.lo += load4_edge((const T*)e.bias, col, n, false);
-    v.hi += load4_edge((const T*)e.bias, col + 4, n, false);
+  if (wave) {
+    sums[wave - 1][0][lane] = v.lo;
+    sums[wave - 1][1][lane] = v.hi;
   }
-  if (e.aux || e.act != DGPRF_ACT_NONE) {
-    with_act(e.act, [&](auto act) {
-      constexpr int ACT = decltype(act)::value;
-      F8 z;
+  __syncthreads();
+  if (wave || !live) return;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        z.lo[c] = saved_of<ACT>(v.lo[c]);
-        z.hi[c] = saved_of<ACT>(v.hi[c]);
-        v.lo[c] = act_of<T, ACT>(v.lo[c]);
-        v.hi[c] = act_of<T, ACT>(v.hi[c]);
-      }
-      if (e.aux) store8((T*)e.aux + row * e.ldaux, col, (int)e.ldaux, true, z);
-    });
+  for (int w = 0; w < 3; ++w) {
+    v.lo += sums[w][0][lane];
+    v.hi += sums[w][1][lane];
   }
-  if (e.drop.thr) v = drop8(v, drop_words(e.drop, drop_sub(e.drop), (uint64_t)q), e.drop);
+  F8 b{f4zero(), f4zero()};
+  if (e.bias) b = load8((const T*)e.bias, col, n, false);
+  const uint64_t sub = e.drop.thr ? drop_sub(e.drop) : 0;
+  with_act(e.act, [&](auto act) { v = value_of<T, decltype(act)::value>(e, row, col, sub, v, b); });
   if (e.res) {
-    const F8 r = load8((const T*)e.res + row * e.ldr, col, n, e.vec_r == 2);
+    const F8 r = load8((const T*)e.res + row * e.ldr, col, n, e.vec_r);
     v.lo += r.lo;
     v.hi += r.hi;
   }
-  store8((T*)e.y + row * e.ldy, col, n, e.vec_y == 2, v);
+  store8((T*)e.y + row * e.ldy, col, n, e.vec_y, v);
 }
 
 // ---------------------------------------------------------------- few rows
@@ -317,7 +270,7 @@ __global__ __launch_bounds__(256) void k_dropout(const T* __restrict__ x, int64_
 }
 
 // ---------------------------------------------------------------- choices
-bool aligned(const void* p, int64_t ld, int64_t cols, int es, int bytes) {
+int aligned(const void* p, int64_t ld, int64_t cols, int es, int bytes) {
   return (uintptr_t)p % bytes == 0 && ld * es % bytes == 0 && cols * es % bytes == 0;
 }
 // rows of 16-byte pieces: what the tiled product reads in place
@@ -333,20 +286,20 @@ constexpr int64_t kMaxWidth = 1 << 20;  // a tile's rows stay within a buffer de
 Shape shape_of(int64_t I, int64_t J, int64_t K, int es) {
   Shape s;
   const int64_t big = cdiv(I, 256) * cdiv(J, 256);
-  s.tile = I <= 32 ? TILE_32 : big >= 160 ? TILE_256 : TILE_128;
-  const int bm = s.tile == TILE_256 ? 256 : s.tile == TILE_128 ? 128 : 32, bn = s.tile == TILE_256 ? 256 : 128;
-  s.n_mt = (int)cdiv(I, bm);
-  s.n_nt = (int)cdiv(J, bn);
-  s.stages = (int)cdiv(K * es, 128);
+  s.tile = es == 4 ? TILE_64 : I <= 32 ? TILE_32 : big >= 160 ? TILE_256 : TILE_128;
+  const TileShape ts = kTiles[s.tile];
+  s.n_mt = (int)cdiv(I, ts.bm);
+  s.n_nt = (int)cdiv(J, ts.bn);
+  s.stages = (int)cdiv(K * es, ts.kb);
   const int64_t tiles = (int64_t)s.n_mt * s.n_nt;
   int64_t want = tiles < 256 ? cdiv(512, tiles) : 1;
-  want = std::min<int64_t>({want, std::max(1, s.stages / 4), 32});
+  want = std::min<int64_t>({want, std::max(1, s.stages * ts.kb / 512), 32});
   s.stages_split = (int)cdiv(s.stages, want);
   s.splits = (int)cdiv(s.stages, s.stages_split);
   return s;
 }
 int64_t part_bytes(const Shape& s, int64_t I, int64_t J) {
-  return s.splits > 1 ? up((int64_t)s.splits * I * up(J, 4) * 4, 256) : 0;
+  return s.splits > 1 ? up((int64_t)s.splits * I * up(J, 8) * 4, 256) : 0;
 }
 
 // parts of K for the few-row kernel: enough workgroups to keep the memory busy
@@ -407,7 +360,7 @@ hipError_t join(int dtype, const float* part, int64_t ldp, int parts, int64_t ro
                 hipStream_t s) {
   return with_type(dtype, [&](auto* t) {
     typedef DENSE_T(t) T;
-    hipLaunchKernelGGL((k_join<T>), dim3((unsigned)cdiv(rows * e.groups, 256)), dim3(256), 0, s, part, ldp,
+    hipLaunchKernelGGL((k_join<T>), dim3((unsigned)cdiv(rows * e.groups, 64)), dim3(256), 0, s, part, ldp,
                        parts, rows, e);
     return hipGetLastError();
   });
@@ -451,7 +404,7 @@ hipError_t product(int dtype, int layout, const void* A, int64_t lda, const void
   a.stages = s.stages;
   a.stages_split = s.stages_split;
   a.part = s.splits > 1 ? part : nullptr;
-  a.ldp = up(J, 4);
+  a.ldp = up(J, 8);
   hipError_t err = gemm(dtype, layout, s, a, e, st);
   if (err == hipSuccess && a.part) err = join(dtype, part, a.ldp, s.splits, I, e, st);
   return err;
@@ -463,7 +416,7 @@ EpiDev epi_plain(void* y, int64_t n, int es) {
   e.ldy = n;
   e.n = (int)n;
   e.groups = (int)cdiv(n, 8);
-  e.vec_y = aligned(y, n, n, es, 8 * es) ? 2 : aligned(y, n, n, es, 4 * es) ? 1 : 0;
+  e.vec_y = aligned(y, n, n, es, 16);
   return e;
 }
 
@@ -491,12 +444,12 @@ hipError_t forward(const dgprf_linear_t& a, Scratch& sc, hipStream_t st, bool ru
   e.ldr = a.ldr;
   e.ldaux = up(n, 8);
   e.act = a.act;
-  e.vec_r = aligned(a.res, a.ldr, 0, es, 8 * es) ? 2 : aligned(a.res, a.ldr, 0, es, 4 * es) ? 1 : 0;
+  e.vec_r = aligned(a.res, a.ldr, 0, es, 16);
   e.drop = drop_dev(a.drop_thr, a.seed, a.sub, a.step);
   if (m <= kRowsMax) {
     int k_part, parts;
     rows_shape(n, k, es, &k_part, &parts);
-    const int64_t ldp = up(n, 4);
+    const int64_t ldp = up(n, 8);
     float* part = (float*)sc.take((int64_t)parts * m * ldp * 4);
     if (!run) return hipSuccess;
     const bool vec = in_place(a.w, a.ldw, n, es);
@@ -552,7 +505,7 @@ hipError_t backward(const dgprf_linear_grad_t& a, Scratch& sc, hipStream_t st, b
     d.N = (int)n;
     d.groups = (int)cdiv(n, 8);
     d.act = a.act;
-    d.vec = aligned(a.dy, a.lddy, 0, es, 8 * es) ? 1 : 0;
+    d.vec = aligned(a.dy, a.lddy, 0, es, 16);
     d.drop = drop_dev(a.drop_thr, a.seed, a.sub, a.step);
     const int64_t strips = cdiv(d.groups, 64);
     const int64_t want = std::max<int64_t>(1, std::min<int64_t>(cdiv(2048, strips), cdiv(m, 16)));
@@ -694,11 +647,9 @@ int dgprf_dropout(int32_t dtype, const void* x, int64_t rows, int64_t n, int64_t
   if (!x || !y) return DGPRF_E_ARG;
   const int64_t groups = cdiv(n, 8);
   if (rows > ((int64_t)1 << 39) / groups) return DGPRF_E_SHAPE;
-  const int es = elem_size(dtype);
   const int64_t total = rows * groups;
-  const bool flat = n % 8 == 0 && (rows == 1 || ldx == n) && (uintptr_t)x % (8 * es) == 0 &&
-                    (uintptr_t)y % (8 * es) == 0 &&
-                    (!res || ((rows == 1 || ldr == n) && (uintptr_t)res % (8 * es) == 0));
+  const bool flat = n % 8 == 0 && (rows == 1 || ldx == n) && (uintptr_t)x % 16 == 0 &&
+                    (uintptr_t)y % 16 == 0 && (!res || ((rows == 1 || ldr == n) && (uintptr_t)res % 16 == 0));
   const DropDev d = drop_dev(drop_thr, seed, sub, step);
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   return hip_rc(with_type(dtype, [&](auto* t) {

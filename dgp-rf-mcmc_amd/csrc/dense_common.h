@@ -167,23 +167,13 @@ struct EpiDev {
   int64_t ldr, ldy, ldaux;
   int32_t n, act;
   int32_t groups;    // ceil(n / 8)
-  int32_t vec_y, vec_r;  // rows of y / res are aligned for 4 elements at a time
+  int32_t vec_y, vec_r;  // rows of y / res allow 16-byte accesses
   DropDev drop;
 };
 
+// columns col .. col + 3 of a row of n, element by element
 template <class T>
-__device__ __forceinline__ f4 load4(const T* p) {
-  const typename Vec<T>::v4 v = *reinterpret_cast<const typename Vec<T>::v4*>(p);
-  return __builtin_convertvector(v, f4);
-}
-template <class T>
-__device__ __forceinline__ void store4(T* p, f4 v) {
-  *reinterpret_cast<typename Vec<T>::v4*>(p) = __builtin_convertvector(v, typename Vec<T>::v4);
-}
-// columns col .. col + 3 of a row of n; aligned: the row allows 4-element accesses
-template <class T>
-__device__ __forceinline__ f4 load4_edge(const T* row, int col, int n, bool aligned) {
-  if (aligned && col + 4 <= n) return load4(row + col);
+__device__ __forceinline__ f4 load4_edge(const T* row, int col, int n) {
   f4 v = f4zero();
 #pragma unroll
   for (int c = 0; c < 4; ++c)
@@ -191,14 +181,101 @@ __device__ __forceinline__ f4 load4_edge(const T* row, int col, int n, bool alig
   return v;
 }
 template <class T>
-__device__ __forceinline__ void store4_edge(T* row, int col, int n, bool aligned, f4 v) {
-  if (aligned && col + 4 <= n) {
-    store4(row + col, v);
-    return;
-  }
+__device__ __forceinline__ void store4_edge(T* row, int col, int n, f4 v) {
 #pragma unroll
   for (int c = 0; c < 4; ++c)
     if (col + c < n) row[col + c] = (T)v[c];
+}
+
+// ---------------------------------------------------------------- eight columns of a row
+struct F8 {
+  f4 lo, hi;
+};
+template <class T>
+__device__ __forceinline__ F8 load8_whole(const T* p) {  // 16-byte aligned
+  F8 v;
+  if constexpr (sizeof(T) == 4) {
+    v.lo = *reinterpret_cast<const f4*>(p);
+    v.hi = *reinterpret_cast<const f4*>(p + 4);
+  } else {
+    const typename Vec<T>::v8 x = *reinterpret_cast<const typename Vec<T>::v8*>(p);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      v.lo[c] = (float)x[c];
+      v.hi[c] = (float)x[c + 4];
+    }
+  }
+  return v;
+}
+template <class T>
+__device__ __forceinline__ void store8_whole(T* p, const F8& v) {  // 16-byte aligned
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<f4*>(p) = v.lo;
+    *reinterpret_cast<f4*>(p + 4) = v.hi;
+  } else {
+    typename Vec<T>::v8 x;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      x[c] = (T)v.lo[c];
+      x[c + 4] = (T)v.hi[c];
+    }
+    *reinterpret_cast<typename Vec<T>::v8*>(p) = x;
+  }
+}
+// columns col .. col + 7 of a row of n; aligned: the row allows 16-byte accesses
+template <class T>
+__device__ __forceinline__ F8 load8(const T* row, int col, int n, bool aligned) {
+  if (aligned && col + 8 <= n) return load8_whole(row + col);
+  F8 v;
+  v.lo = load4_edge(row, col, n);
+  v.hi = load4_edge(row, col + 4, n);
+  return v;
+}
+template <class T>
+__device__ __forceinline__ void store8(T* row, int col, int n, bool aligned, const F8& v) {
+  if (aligned && col + 8 <= n) {
+    store8_whole(row + col, v);
+  } else {
+    store4_edge(row, col, n, v.lo);
+    store4_edge(row, col + 4, n, v.hi);
+  }
+}
+__device__ __forceinline__ F8 drop8(F8 v, const u32x4& w, const DropDev& d) {
+  v.lo[0] = drop_lo(v.lo[0], w.x, d);
+  v.lo[1] = drop_hi(v.lo[1], w.x, d);
+  v.lo[2] = drop_lo(v.lo[2], w.y, d);
+  v.lo[3] = drop_hi(v.lo[3], w.y, d);
+  v.hi[0] = drop_lo(v.hi[0], w.z, d);
+  v.hi[1] = drop_hi(v.hi[1], w.z, d);
+  v.hi[2] = drop_lo(v.hi[2], w.w, d);
+  v.hi[3] = drop_hi(v.hi[3], w.w, d);
+  return v;
+}
+
+// s m a(v + b) of eight columns of a row; stores what backward needs of v + b
+template <class T, int ACT>
+__device__ __forceinline__ F8 value_of(const EpiDev& e, int64_t row, int col, uint64_t sub, F8 v, const F8& b) {
+  v.lo += b.lo;
+  v.hi += b.hi;
+  if constexpr (ACT != DGPRF_ACT_NONE) {
+    if (e.aux) {
+      F8 z;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        z.lo[c] = saved_of<ACT>(v.lo[c]);
+        z.hi[c] = saved_of<ACT>(v.hi[c]);
+      }
+      store8_whole((T*)e.aux + row * e.ldaux + col, z);
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      v.lo[c] = act_of<T, ACT>(v.lo[c]);
+      v.hi[c] = act_of<T, ACT>(v.hi[c]);
+    }
+  }
+  if (e.drop.thr)
+    v = drop8(v, drop_words(e.drop, sub, (uint64_t)row * (uint32_t)e.groups + (uint32_t)(col >> 3)), e.drop);
+  return v;
 }
 
 // ---------------------------------------------------------------- tiled product
@@ -216,7 +293,11 @@ struct GemmArgs {
 };
 
 enum { LAYOUT_NN = 0, LAYOUT_NT = 1, LAYOUT_TN = 2 };  // forward, dx, dW
-enum { TILE_256 = 0, TILE_128 = 1, TILE_32 = 2 };
+enum { TILE_256 = 0, TILE_256N = 1, TILE_128 = 2, TILE_64 = 3, TILE_32 = 4, TILES = 5 };
+struct TileShape {
+  int bm, bn, kb;  // rows, columns, bytes of K of a stage
+};
+constexpr TileShape kTiles[TILES] = {{256, 256, 128}, {256, 128, 64}, {128, 128, 64}, {64, 64, 128}, {32, 128, 128}};
 
 // one instantiation per element type (dense_<type>.hip): layout, tile, and epilogue (part == null:
 // the linear epilogue e; otherwise partial sums)

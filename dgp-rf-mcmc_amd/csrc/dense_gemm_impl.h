@@ -2,13 +2,14 @@
 // products of a layer: forward z = x W (A[i][k], B[k][j]), dx = dz W^T (A[i][k], B[j][k]) and
 // dW = x^T dz (A[k][i], B[k][j]); x, W and dz stay in their row-major layouts.
 //
-// A workgroup computes a BM x BN tile; a stage is 128 bytes of K (64 16-bit or 32 fp32 elements).
-// Both operands' stages go from memory to LDS without passing registers (16-byte buffer loads with
-// the LDS destination), double-buffered: stage t + 1 is in flight while stage t is multiplied, one
-// barrier per stage.  The LDS image of a load is linear in the lane, so bank conflicts are avoided
-// by permuting which 16 bytes of the source each lane fetches (XOR on the 16-byte index).
-//  * K-contiguous operand: rows of 128 bytes, slot = chunk ^ (row & 7); a lane's MFMA fragment is
-//    one ds_read_b128.
+// A workgroup of four waves computes a BM x BN tile; a stage is KB bytes of K (64 or 128; 64 bytes
+// are 32 16-bit or 16 fp32 elements, one step of the matrix instructions).  Both operands' stages go
+// from memory to LDS without passing registers (16-byte buffer loads with the LDS destination) into
+// ST buffers, one barrier per stage.  The LDS
+// image of a load is linear in the lane, so bank conflicts are avoided by permuting which 16 bytes of
+// the source each lane fetches (XOR on the 16-byte index).
+//  * K-contiguous operand: rows of KB bytes, the slots permuted so that eight neighbouring rows' equal
+//    chunks fall on all banks; a lane's MFMA fragment is one ds_read_b128.
 //  * K-strided operand: rows of one k.  16-bit fragments come from two ds_read_b64_tr_b16 (a 16-lane
 //    group reads a 4 k x 16 column block and gets it transposed); fp32 fragments from four b32 reads.
 // The MFMA's first operand is the B fragment, so D holds C transposed: a lane has four consecutive
@@ -17,7 +18,9 @@
 // Edges: rows / columns past I, J fetch the last row again or zeros, and are not stored; K past the
 // end fetches zeros (offsets past the buffer descriptor's range read 0 without an access).
 #pragma once
-#include <type_traits>
+
+#include <algorithm>
+#include <atomic>
 
 #include "dense_common.h"
 
@@ -29,10 +32,21 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 constexpr uint32_t kOob = DGPRF_OOB;
 
-__device__ __forceinline__ rsrc_t rsrc_of(const void* p, int64_t bytes) {
-  const int n = bytes > 0x7FFFFFF0ll ? 0x7FFFFFF0 : bytes < 0 ? 0 : (int)bytes;
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, n, 0x00020000);
+// Raw buffer descriptor (base, 0 | range in bytes | data format), in scalar registers.
+typedef uint32_t desc_t __attribute__((ext_vector_type(4)));
+// 16 bytes a lane from the descriptor's `off` (zeros past its range) to LDS at `to` + 16 lane.  Written
+// as an instruction because the compiler, which cannot tell the buffers apart, would wait for every
+// load in flight before each transposing LDS read; it has no destination register, and the waits are
+// the loop's own (wait_loads).  M0 takes a wait state before the load reads it.
+__device__ __forceinline__ void load_to_lds(desc_t d, uint32_t off, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(to), "v"(off), "s"(d)
+               : "memory", "m0");
 }
+
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // XOR of the 16-byte index within row k of a K-strided stage, C columns wide
 template <class T, int C>
@@ -43,41 +57,54 @@ __device__ __forceinline__ int swz_strided(int k) {
   else return 2 * ((k >> 3) & 1);
 }
 
+// slot permutation of a K-contiguous row
+template <int KB>
+__device__ __forceinline__ int swz_row(int r) {
+  return KB == 64 ? (r >> 1) & 3 : r & 7;
+}
+
 // One operand's stages: R rows (KC) or columns of the tile, NT threads
-template <class T, bool KC, int R, int NT>
+template <class T, bool KC, int R, int KB, int NT>
 struct Stage {
   static constexpr int CE = 16 / (int)sizeof(T);   // elements of a 16-byte chunk
-  static constexpr int BK = 128 / (int)sizeof(T);  // K of a stage
-  static constexpr int LOADS = R * 8 / NT;
-  static constexpr int BYTES = R * 128;
+  static constexpr int BK = KB / (int)sizeof(T);   // K of a stage
+  static constexpr int CPK = KB / 16;              // chunks of a K-contiguous row
   static constexpr int CPR = R / CE;               // chunks of a K-strided row
-  static_assert(LOADS >= 1 && R * 8 % NT == 0, "tile too small for the workgroup");
+  static constexpr int LOADS = R * CPK / NT;
+  static constexpr int BYTES = R * KB;
+  static_assert(LOADS >= 1 && R * CPK % NT == 0, "tile too small for the workgroup");
+  static_assert(NT / CPK % 8 == 0, "a lane's chunk must be the same in each of its loads");
   uint32_t off[LOADS];
-  const char* base;
-  int64_t step;   // bytes between stages
-  int64_t range;  // K-strided: bytes from base to the operand's end; KC: of the tile's rows
-  int k_end, kk;  // KC: K, and this lane's first chunk's element offset
+  desc_t desc;         // of the stage being loaded
+  uint32_t step_lo, step_hi;  // bytes between stages
+  uint32_t full, tail;  // bytes that a stage, and the last one with data, may reach over
+  int last, k_last;    // its number; KC: K in it
+  int kk;              // KC: element offset of this lane's chunk
 
-  // rows r0 .. of `rows` (KC), or columns r0 .. of `cols` readable ones
-  __device__ __forceinline__ void init(const void* p, int64_t ld, int r0, int rows, int cols, int K,
-                                       int tid) {
+  // rows r0 .. of `rows` (KC), or columns r0 .. of `cols` readable ones; stages t0 .. t1 - 1 of K
+  __device__ __forceinline__ void init(const void* p, int64_t ld, int r0, int rows, int cols, int K, int t0,
+                                       int t1, int tid) {
+    const char* base = (const char*)p;
+    const int end = (K + BK - 1) / BK - 1;
+    int64_t f, t, step;
+    k_last = K - end * BK;
     if constexpr (KC) {
-      base = (const char*)p + (int64_t)r0 * ld * sizeof(T);
-      step = 128;
-      const int last = rows - 1 - r0;
-      range = ((int64_t)min(last, R - 1) * ld + K) * sizeof(T);
-      k_end = K;
+      base += (int64_t)r0 * ld * sizeof(T);
+      step = KB;
+      const int lr = min(rows - 1 - r0, R - 1);
+      f = (int64_t)lr * ld + BK;
+      t = (int64_t)lr * ld + k_last;
 #pragma unroll
       for (int j = 0; j < LOADS; ++j) {
-        const int q = tid + NT * j, r = q >> 3, c = (q & 7) ^ (r & 7);
-        off[j] = (uint32_t)(min(r, last) * (int)ld + c * CE) * (uint32_t)sizeof(T);
+        const int q = tid + NT * j, r = q / CPK, c = (q % CPK) ^ swz_row<KB>(r);
+        off[j] = (uint32_t)(min(r, lr) * (int)ld + c * CE) * (uint32_t)sizeof(T);
       }
-      kk = ((tid & 7) ^ ((tid >> 3) & 7)) * CE;  // the same for every j: NT / 8 is a multiple of 8
+      kk = ((tid % CPK) ^ swz_row<KB>(tid / CPK)) * CE;
     } else {
-      base = (const char*)p + (int64_t)r0 * sizeof(T);
+      base += (int64_t)r0 * sizeof(T);
       step = (int64_t)BK * ld * sizeof(T);
-      range = ((int64_t)(K - 1) * ld + (cols - r0)) * sizeof(T);
-      k_end = 0;
+      f = (int64_t)(BK - 1) * ld + (cols - r0);
+      t = (int64_t)(k_last - 1) * ld + (cols - r0);
       kk = 0;
 #pragma unroll
       for (int j = 0; j < LOADS; ++j) {
@@ -85,37 +112,51 @@ struct Stage {
         off[j] = r0 + c * CE < cols ? (uint32_t)(k * (int)ld + c * CE) * (uint32_t)sizeof(T) : kOob;
       }
     }
+    if (t1 - 1 < end) {  // this part of K ends before
+      t = f;
+      k_last = BK;
+    }
+    // wave-uniform all, and kept in scalar registers, where next() and the loads need them
+    full = uniform((uint32_t)f * (uint32_t)sizeof(T));  // below 2^31 by the limits on widths
+    tail = uniform((uint32_t)t * (uint32_t)sizeof(T));
+    last = uniform(min(t1 - 1, end));
+    k_last = uniform(k_last);
+    step_lo = uniform((uint32_t)step);
+    step_hi = uniform((uint32_t)(step >> 32));
+    const uint64_t at = (uint64_t)base + (uint64_t)((t0 - 1) * step);  // next() goes to t0
+    desc[0] = uniform((uint32_t)at);
+    desc[1] = uniform((uint32_t)(at >> 32));
+    desc[2] = 0;
+    desc[3] = 0x00020000u;
   }
-  // stage t to LDS at `to` (wave-uniform: the wave's first 16-byte slot)
-  __device__ __forceinline__ void load(int t, char* to) const {
-    const int64_t at = (int64_t)t * step;
-    const rsrc_t r = rsrc_of(base + at, range - at);
-    if (KC && (t + 1) * BK > k_end) {
-      const bool in = t * BK + kk < k_end;
+  // To stage t, the one after the last time's.  Its loads (load) go to `to` (wave-uniform: the wave's
+  // first 16-byte slot); past the last stage, and of K past the end, they bring zeros, without an
+  // access.  A few scalar instructions: they run between matrix instructions.
+  __device__ __forceinline__ void next(int t) {
+    const uint64_t at = ((uint64_t)desc[1] << 32 | desc[0]) + ((uint64_t)step_hi << 32 | step_lo);
+    desc[0] = (uint32_t)at;
+    desc[1] = (uint32_t)(at >> 32);
+    desc[2] = t < last ? full : t == last ? tail : 0u;
+    if (KC && t == last && k_last < BK) {
 #pragma unroll
-      for (int j = 0; j < LOADS; ++j)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(to + j * NT * 16), 16,
-                                                 in ? off[j] : kOob, 0, 0, 0);
-    } else {
-#pragma unroll
-      for (int j = 0; j < LOADS; ++j)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(to + j * NT * 16), 16, off[j], 0, 0,
-                                                 0);
+      for (int j = 0; j < LOADS; ++j) off[j] = kk < k_last ? off[j] : kOob;
     }
   }
+  __device__ __forceinline__ void load(int j, uint32_t to) const { load_to_lds(desc, off[j], to + j * NT * 16); }
 };
 
 // A fragment: 16 bytes; 16-bit: k = 8 g + e of 32, fp32: k = 4 g + e of 16 (g = lane >> 4), row or
 // column lane & 15.  NF fragments 16 apart, starting at w0 of the tile's R.
-template <class T, bool KC, int R, int NF>
+template <class T, bool KC, int R, int KB, int NF>
 struct Frags {
   typedef typename std::conditional<sizeof(T) == 4, f4, typename Vec<T>::v8>::type frag;
-  uint32_t at[KC ? 2 : NF];
+  static constexpr int KS = KB / 64;  // steps of a stage
+  uint32_t at[KC ? KS : NF];
   __device__ __forceinline__ void init(int w0, int lane) {
     const int g = lane >> 4, i = lane & 15;
     if constexpr (KC) {
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) at[ks] = (w0 + i) * 128 + (((ks * 4 + g) ^ (i & 7)) * 16);
+      for (int ks = 0; ks < KS; ++ks) at[ks] = (w0 + i) * KB + (((ks * 4 + g) ^ swz_row<KB>(i)) * 16);
     } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
       for (int f = 0; f < NF; ++f) {
@@ -132,7 +173,7 @@ struct Frags {
   }
   __device__ __forceinline__ frag read(const char* lds, int ks, int f) const {
     if constexpr (KC) {
-      return *reinterpret_cast<const frag*>(lds + at[ks] + f * 2048);
+      return *reinterpret_cast<const frag*>(lds + at[ks] + f * 16 * KB);
     } else if constexpr (sizeof(T) == 4) {
       frag v;
 #pragma unroll
@@ -152,12 +193,11 @@ struct Frags {
   }
 };
 
+// part p of a step (fp32: of four, k = 4 g + p)
 template <class T, class F>
-__device__ __forceinline__ f4 mma(F b, F a, f4 c) {
+__device__ __forceinline__ f4 mma(F b, F a, f4 c, int p) {
   if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int s = 0; s < 4; ++s) c = mfma16(b[s], a[s], c);
-    return c;
+    return mfma16(b[p], a[p], c);
   } else if constexpr (std::is_same<T, bf16_t>::value) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, a, c, 0, 0, 0);
   } else {
@@ -165,19 +205,100 @@ __device__ __forceinline__ f4 mma(F b, F a, f4 c) {
   }
 }
 
-// vmcnt(0), leaving the other counters alone
-#define DENSE_WAIT_LOADS() __builtin_amdgcn_s_waitcnt(0x0F70)
+// LDS reads of a fragment
+template <class T, bool KC>
+constexpr int reads() {
+  return KC ? 1 : sizeof(T) == 4 ? 4 : 2;
+}
 
-template <class T, bool AKC, bool BKC, int BM, int BN, int WM, int WN, bool PART>
-__global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void k_dense(const GemmArgs a,
-                                                                    const EpiDev e) {
+// The same into accumulation registers: with 64 accumulators (256 registers) the compiler moves them
+// between the two register files in the loop; as an operand of this instruction one stays where it is.
+// Its result is next read by the same instruction 64 of them later, or after settle().
+template <class T, class F>
+__device__ __forceinline__ void mma_acc(F b, F a, f4& c) {
+  if constexpr (std::is_same<T, bf16_t>::value)
+    asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(b), "v"(a));
+  else
+    asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(b), "v"(a));
+}
+// ... and a load to LDS behind it, which it gives M0's wait state
+template <class T, class F>
+__device__ __forceinline__ void mma_acc_load(F b, F a, f4& c, desc_t d, uint32_t off, uint32_t to, uint32_t more) {
+  if constexpr (std::is_same<T, bf16_t>::value)
+    asm volatile("s_add_u32 m0, %5, %6\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, %0\n\t"
+                 "buffer_load_dwordx4 %3, %4, 0 offen lds"
+                 : "+a"(c)
+                 : "v"(b), "v"(a), "v"(off), "s"(d), "s"(to), "s"(more)
+                 : "memory", "m0", "scc");
+  else
+    asm volatile("s_add_u32 m0, %5, %6\n\tv_mfma_f32_16x16x32_f16 %0, %1, %2, %0\n\t"
+                 "buffer_load_dwordx4 %3, %4, 0 offen lds"
+                 : "+a"(c)
+                 : "v"(b), "v"(a), "v"(off), "s"(d), "s"(to), "s"(more)
+                 : "memory", "m0", "scc");
+}
+// the last matrix instructions' results are readable (16 passes at most are in flight)
+template <int MI, int NI>
+__device__ __forceinline__ void settle(f4 (&acc)[MI][NI]) {
+  asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NI; ++j) asm volatile("" : "+a"(acc[i][j]));
+}
+
+// LDS that a wave's sub-tile takes on its way out, CR rows at a time; the pitch spreads the rows of a
+// write over the banks
+template <int BM, int BN, int WM, int WN>
+struct Turned {
+  static constexpr int CR = WM < 64 ? WM : 64, PITCH = WN + 4, BYTES = CR * PITCH * 4;
+};
+// Eight columns of a row that allows 16-byte accesses: n is a multiple of 8, or of 4 in fp32, where the
+// last group may be half there.
+template <class T>
+__device__ __forceinline__ F8 load8_edge4(const T* row, int col, int n) {
+  if constexpr (sizeof(T) == 4) {
+    F8 v;
+    v.lo = *reinterpret_cast<const f4*>(row + col);
+    v.hi = col + 4 < n ? *reinterpret_cast<const f4*>(row + col + 4) : f4zero();
+    return v;
+  } else {
+    return load8_whole(row + col);
+  }
+}
+template <class T>
+__device__ __forceinline__ void store8_edge4(T* row, int col, int n, const F8& v) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<f4*>(row + col) = v.lo;
+    if (col + 4 < n) *reinterpret_cast<f4*>(row + col + 4) = v.hi;
+  } else {
+    store8_whole(row + col, v);
+  }
+}
+// the wave's LDS accesses before are done before those after
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// all LDS reads done and at most N loads outstanding
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | ((N >> 4) << 14));
+}
+
+template <class T, bool AKC, bool BKC, int BM, int BN, int WM, int WN, int KB, int ST, int OCC, bool PART>
+__global__ __launch_bounds__(256, OCC) void k_dense(const GemmArgs a, const EpiDev e) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host pass needs the stub alone
-  constexpr int NT = BM / WM * (BN / WN) * 64, MI = WM / 16, NI = WN / 16;
-  typedef Stage<T, AKC, BM, NT> SA;
-  typedef Stage<T, BKC, BN, NT> SB;
-  typedef Frags<T, AKC, BM, MI> FA;
-  typedef Frags<T, BKC, BN, NI> FB;
-  static_assert(NI % 2 == 0, "the epilogue shares a generator call between two column blocks");
+  constexpr int NT = 256, MI = WM / 16, NI = WN / 16;
+  static_assert(BM / WM * (BN / WN) == 4, "four waves");
+  constexpr bool BIG = MI * NI == 64;  // accumulators fill a register file
+  static_assert(!BIG || (MI == 8 && NI == 8 && sizeof(T) == 2 && BM == 256), "turn()'s groups");
+  typedef Stage<T, AKC, BM, KB, NT> SA;
+  typedef Stage<T, BKC, BN, KB, NT> SB;
+  typedef Frags<T, AKC, BM, KB, MI> FA;
+  typedef Frags<T, BKC, BN, KB, NI> FB;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
 
   // XCD-contiguous order (workgroup b runs on XCD b % 8), and within it column sweeps of 8 row
@@ -201,8 +322,9 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void k_dense(const GemmAr
 
   SA sa;
   SB sb;
-  sa.init(a.A, a.lda, i0, a.I, a.Ia, a.Ka, tid);
-  sb.init(a.B, a.ldb, j0, a.J, a.Ja, a.Kb, tid);
+  const int t0 = split * a.stages_split, t1 = min(a.stages, t0 + a.stages_split);
+  sa.init(a.A, a.lda, i0, a.I, a.Ia, a.Ka, t0, t1, tid);
+  sb.init(a.B, a.ldb, j0, a.J, a.Ja, a.Kb, t0, t1, tid);
   FA fa;
   FB fb;
   fa.init(wi, lane);
@@ -214,152 +336,231 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void k_dense(const GemmAr
 #pragma unroll
     for (int j = 0; j < NI; ++j) acc[i][j] = f4zero();
 
-  const int t0 = split * a.stages_split, t1 = min(a.stages, t0 + a.stages_split);
-  char* const lds_a = smem;
-  char* const lds_b = smem + 2 * SA::BYTES;
-  auto issue = [&](int t, int buf) {
-    sa.load(t, lds_a + buf * SA::BYTES + wave * 1024);
-    sb.load(t, lds_b + buf * SB::BYTES + wave * 1024);
-  };
-  auto multiply = [&](int buf) {
-    const char* la = lds_a + buf * SA::BYTES;
-    const char* lb = lds_b + buf * SB::BYTES;
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      typename FB::frag bv[NI];
-#pragma unroll
-      for (int j = 0; j < NI; ++j) bv[j] = fb.read(lb, ks, j);
-#pragma unroll
-      for (int i = 0; i < MI; ++i) {
-        const typename FA::frag av = fa.read(la, ks, i);
-#pragma unroll
-        for (int j = 0; j < NI; ++j) acc[i][j] = mma<T>(bv[j], av, acc[i][j]);
-      }
-    }
-  };
-  auto arrive = [&]() {  // this wave's loads have landed, then everyone's
-    DENSE_WAIT_LOADS();
+  // Steps run one ahead in registers: while step s is multiplied, the fragments of step s + 1 are read
+  // from LDS into the other set.  A new stage's fragments are read after a barrier that says that its
+  // loads have landed; the same barrier says that everyone has read the stage before it, whose buffer
+  // then takes the stage ST later.  Stages past the end load zeros, so every stage has the same loads.
+  constexpr int BUF = SA::BYTES + SB::BYTES, LOADS = SA::LOADS + SB::LOADS, KS = KB / 64;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void*)smem + wave * 1024;
+  typename FA::frag av[2][MI];
+  typename FB::frag bv[2][NI];
+  auto barrier = []() {
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
-  if (t0 < t1) issue(t0, 0);
-  for (int t = t0; t < t1; t += 2) {
-    arrive();
-    if (t + 1 < t1) issue(t + 1, 1);
-    multiply(0);
-    if (t + 1 < t1) {
-      arrive();
-      if (t + 2 < t1) issue(t + 2, 0);
-      multiply(1);
+  auto read_one = [&](int f, int set, int at, int ks) {  // fragment f of a step: B's, then A's
+    if (f < NI) bv[set][f] = fb.read(smem + at + SA::BYTES, ks, f);
+    else av[set][f - NI] = fa.read(smem + at, ks, f - NI);
+  };
+  // One step: its matrix instructions with everything else between them, a little after each.  A wave
+  // issues in order, and a matrix instruction of 16 cycles hides about three others behind it: in a
+  // burst after several of them, the same instructions stand in the way of the next (4096^3 in bf16:
+  // 114 us with groups of four).  Reads take the first three quarters, so that the last of them have
+  // time to land before the next step.  next_at, next_ks: where the other set's fragments are;
+  // new_stage: also load the stage ST later (t + ST) to buffer old.
+  constexpr int PARTS = sizeof(T) == 4 ? 4 : 1, M = MI * NI * PARTS, F = MI + NI, MR = M * 3 / 4;
+  auto run = [&](int set, bool reading, int next_at, int next_ks, bool new_stage, int t, int old) __attribute__((always_inline)) {
+    int f = 0, l = 0;
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      const int p = m / (MI * NI), i = m % (MI * NI) / NI, j = m % NI;  // p: part of the step
+      bool load = new_stage && l < LOADS && m >= (2 * l + 1) * M / LOADS / 2;
+      if constexpr (BIG) {
+        if (load && l < SA::LOADS)
+          mma_acc_load<T>(bv[set][j], av[set][i], acc[i][j], sa.desc, sa.off[l], lds0 + l * NT * 16, old);
+        else if (load)
+          mma_acc_load<T>(bv[set][j], av[set][i], acc[i][j], sb.desc, sb.off[l - SA::LOADS],
+                          lds0 + SA::BYTES + (l - SA::LOADS) * NT * 16, old);
+        else
+          mma_acc<T>(bv[set][j], av[set][i], acc[i][j]);
+      } else {
+        acc[i][j] = mma<T>(bv[set][j], av[set][i], acc[i][j], p);
+      }
+      if (!BIG || !load)
+        while (reading && f < F && m >= f * MR / F) read_one(f++, set ^ 1, next_at, next_ks);
+      while (load) {
+        if (!BIG && l < SA::LOADS) sa.load(l, lds0 + old);
+        else if (!BIG) sb.load(l - SA::LOADS, lds0 + old + SA::BYTES);
+        ++l;
+        if (l == SA::LOADS) sa.next(t + ST + 1);
+        if (l == LOADS) sb.next(t + ST + 1);
+        load = !BIG && l < LOADS && m >= (2 * l + 1) * M / LOADS / 2;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  int cur = 0;  // buffer of stage t
+  // multiplies the last step of stage t (set) while the first of stage t + 1 is read into the other
+  auto turn = [&](int t, int set) __attribute__((always_inline)) {
+    wait_loads<(ST - 2) * LOADS>();
+    barrier();
+    const int old = cur;
+    cur = cur == (ST - 1) * BUF ? 0 : cur + BUF;
+    run(set, true, cur, 0, true, t, old);
+  };
+#pragma unroll
+  for (int i = 0; i < ST; ++i) {
+    sa.next(t0 + i);
+    sb.next(t0 + i);
+#pragma unroll
+    for (int k = 0; k < SA::LOADS; ++k) sa.load(k, lds0 + i * BUF);
+#pragma unroll
+    for (int k = 0; k < SB::LOADS; ++k) sb.load(k, lds0 + i * BUF + SA::BYTES);
+  }
+  sa.next(t0 + ST);
+  sb.next(t0 + ST);
+  wait_loads<(ST - 1) * LOADS>();
+  barrier();
+#pragma unroll
+  for (int f = 0; f < F; ++f) read_one(f, 0, 0, 0);
+  if constexpr (KS == 1) {
+    int t = t0;
+    for (; t + 1 < t1; t += 2) {
+      turn(t, 0);
+      turn(t + 1, 1);
+    }
+    if (t < t1) {
+      wait_loads<0>();
+      run(0, false, 0, 0, false, t, 0);
+    }
+  } else {
+    for (int t = t0; t < t1; ++t) {
+      run(0, true, cur, 1, false, t, 0);
+      turn(t, 1);
     }
   }
+  wait_loads<0>();
+  if constexpr (BIG) settle(acc);
 
-  const int g = lane >> 4, r0 = i0 + wi + (lane & 15), c0 = j0 + wj + 4 * g;
+  const int g = lane >> 4;
   if constexpr (PART) {
+    const int r0 = i0 + wi + (lane & 15), c0 = j0 + wj + 4 * g;
     float* const out = a.part + (int64_t)split * a.I * a.ldp;
 #pragma unroll
-    for (int i = 0; i < MI; ++i) {
-      const int row = r0 + 16 * i;
-      if (row >= a.I) continue;
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int j = 0; j < NI; ++j) {
-        const int col = c0 + 16 * j;
-        if (col < a.J) store4(out + (int64_t)row * a.ldp + col, acc[i][j]);  // ldp % 4 == 0
+        const int row = r0 + 16 * i, col = c0 + 16 * j;
+        if (row < a.I && col < a.ldp) *reinterpret_cast<f4*>(out + (int64_t)row * a.ldp + col) = acc[i][j];
       }
-    }
-    return;
-  }
-
-  const int n = e.n;
-  if (e.bias) {
+  } else {
+    // The wave's sub-tile goes through its own part of LDS, CR rows at a time, so that a lane gets eight
+    // columns of a row (one generator call, one 16-byte access) and neighbouring lanes the row's next
+    // ones: rows of 16 lanes' accesses instead of pieces of 32 bytes, and a loop instead of a body for
+    // every accumulator.  U row groups at a time have their residual loads in flight together.  Rows
+    // that 16-byte accesses do not fit (an odd n) go back to LDS and out column by column.
+    typedef Turned<BM, BN, WM, WN> TU;
+    constexpr int CR = TU::CR, PITCH = TU::PITCH, LPR = WN / 8, RPI = 64 / LPR, IT = CR / RPI;
+    constexpr int U = BIG ? 4 : 2;
+    __syncthreads();  // the stages' LDS is free
+    float* const mine = reinterpret_cast<float*>(smem + wave * TU::BYTES);
+    const uint64_t sub = e.drop.thr ? drop_sub(e.drop) : 0;
+    const int lc = (lane % LPR) * 8, lr = lane / LPR, col = j0 + wj + lc;
+    const bool whole = e.vec_y && (!e.res || e.vec_r);  // n is a multiple of 8 (fp32: of 4) then
+    F8 b{f4zero(), f4zero()};
+    if (e.bias && col < e.n) b = load8((const T*)e.bias, col, e.n, false);
+    auto out = [&](auto chunk) __attribute__((always_inline)) {
+      constexpr int CH = decltype(chunk)::value;
 #pragma unroll
-    for (int j = 0; j < NI; ++j) {
-      const f4 b = load4_edge((const T*)e.bias, c0 + 16 * j, n, false);
+      for (int i = 0; i < CR / 16; ++i)
 #pragma unroll
-      for (int i = 0; i < MI; ++i) acc[i][j] += b;
-    }
-  }
-  if (e.aux || e.act != DGPRF_ACT_NONE) {
-    with_act(e.act, [&](auto act) {
-      constexpr int ACT = decltype(act)::value;
+        for (int j = 0; j < NI; ++j)
+          *reinterpret_cast<f4*>(&mine[(16 * i + (lane & 15)) * PITCH + 16 * j + 4 * g]) = acc[CH * (CR / 16) + i][j];
+      wave_sync();
+      const int row0 = i0 + wi + CH * CR;
+      if (col < e.n)
+        with_act(e.act, [&](auto act) __attribute__((always_inline)) {
+          constexpr int ACT = decltype(act)::value;
+#pragma unroll 1
+          for (int it = 0; it < IT; it += U) {
+            F8 res[U];
+            const int r = it * RPI + lr;
+            if (e.res && whole) {
 #pragma unroll
-      for (int i = 0; i < MI; ++i) {
-        const int row = r0 + 16 * i;
+              for (int u = 0; u < U; ++u)
+                if (row0 + r + u * RPI < a.I)
+                  res[u] = load8_edge4<T>((const T*)e.res + (int64_t)(row0 + r + u * RPI) * e.ldr, col, e.n);
+            }
 #pragma unroll
-        for (int j = 0; j < NI; ++j) {
-          const int col = c0 + 16 * j;
-          if (e.aux && row < a.I && col < n) {
-            f4 z = acc[i][j];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) z[c] = saved_of<ACT>(z[c]);
-            store4((T*)e.aux + (int64_t)row * e.ldaux + col, z);
+            for (int u = 0; u < U; ++u) {
+              const int row = row0 + r + u * RPI;
+              if (row >= a.I) continue;
+              float* p = &mine[(r + u * RPI) * PITCH + lc];
+              F8 v;
+              v.lo = *reinterpret_cast<const f4*>(p);
+              v.hi = *reinterpret_cast<const f4*>(p + 4);
+              v = value_of<T, ACT>(e, row, col, sub, v, b);
+              if (whole) {
+                if (e.res) {
+                  v.lo += res[u].lo;
+                  v.hi += res[u].hi;
+                }
+                store8_edge4<T>((T*)e.y + (int64_t)row * e.ldy, col, e.n, v);
+              } else {
+                *reinterpret_cast<f4*>(p) = v.lo;
+                *reinterpret_cast<f4*>(p + 4) = v.hi;
+              }
+            }
           }
-#pragma unroll
-          for (int c = 0; c < 4; ++c) acc[i][j][c] = act_of<T, ACT>(acc[i][j][c]);
-        }
+        });
+      wave_sync();
+      if (!whole) {
+        const int width = min(WN, e.n - j0 - wj), rows = min(CR, a.I - row0);
+        for (int r = lane / WN; r < rows; r += 64 / WN > 0 ? 64 / WN : 1)
+          for (int c = lane % WN; c < width; c += 64) {
+            float v = mine[r * PITCH + c];
+            if (e.res) v += (float)((const T*)e.res)[(int64_t)(row0 + r) * e.ldr + j0 + wj + c];
+            ((T*)e.y)[(int64_t)(row0 + r) * e.ldy + j0 + wj + c] = (T)v;
+          }
+        wave_sync();
       }
-    });
-  }
-  const uint64_t sub = e.drop.thr ? drop_sub(e.drop) : 0;
-#pragma unroll
-  for (int i = 0; i < MI; ++i) {
-    const int row = r0 + 16 * i;
-    if (e.drop.thr) {
-      // lanes g and g ^ 1 hold the halves of the same eight columns: in each pair of column blocks
-      // the even one makes the words of the first block, the odd one of the second, then they swap
-#pragma unroll
-      for (int j = 0; j < NI; j += 2) {
-        const int col = c0 + 16 * (j + (g & 1));
-        const u32x4 w = drop_words(e.drop, sub, (uint64_t)row * (uint32_t)e.groups + (uint32_t)(col >> 3));
-        const auto p = __builtin_amdgcn_permlane16_swap(w.x, w.z, false, false);
-        const auto q = __builtin_amdgcn_permlane16_swap(w.y, w.w, false, false);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          f4& v = acc[i][j + h];
-          v[0] = drop_lo(v[0], p[h], e.drop);
-          v[1] = drop_hi(v[1], p[h], e.drop);
-          v[2] = drop_lo(v[2], q[h], e.drop);
-          v[3] = drop_hi(v[3], q[h], e.drop);
-        }
-      }
-    }
-    if (row >= a.I) continue;
-    const T* res = (const T*)e.res + (int64_t)row * e.ldr;
-    T* y = (T*)e.y + (int64_t)row * e.ldy;
-#pragma unroll
-    for (int j = 0; j < NI; ++j) {
-      const int col = c0 + 16 * j;
-      if (col >= n) continue;
-      f4 v = acc[i][j];
-      if (e.res) v += load4_edge(res, col, n, e.vec_r);
-      store4_edge(y, col, n, e.vec_y, v);
-    }
+    };
+    out(std::integral_constant<int, 0>());
+    if constexpr (WM / CR == 2) out(std::integral_constant<int, 1>());
+    static_assert(WM / CR <= 2, "chunks of a wave's rows");
   }
 #endif
 }
 
-template <class T, bool AKC, bool BKC, int BM, int BN, int WM, int WN>
-hipError_t launch_tile(GemmArgs a, const EpiDev& e, hipStream_t s) {
-  constexpr int NT = BM / WM * (BN / WN) * 64;
-  const size_t lds = 2 * (BM + BN) * 128;
+// Dynamic LDS above 64 KiB is asked for once per kernel and device (the call costs a launch's time).
+inline void allow_lds(const void* fn, size_t bytes, std::atomic<uint64_t>& done) {
+  if (bytes <= 65536) return;
+  int dev = 0;
+  (void)hipGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return;
+  dgprf::set_lds_limit(fn, bytes);
+  done.fetch_or(bit, std::memory_order_relaxed);
+}
+
+template <class T, bool AKC, bool BKC, int BM, int BN, int WM, int WN, int KB, int ST, int OCC>
+hipError_t launch_tile(const GemmArgs& a, const EpiDev& e, hipStream_t s) {
+  const size_t lds = std::max(ST * (BM + BN) * KB, 4 * Turned<BM, BN, WM, WN>::BYTES);
   const dim3 grid((unsigned)(a.n_mt * a.n_nt * a.splits));
   if (a.part) {
-    const auto fn = &k_dense<T, AKC, BKC, BM, BN, WM, WN, true>;
-    dgprf::set_lds_limit((const void*)fn, lds);
-    hipLaunchKernelGGL(fn, grid, dim3(NT), lds, s, a, e);
+    const auto fn = &k_dense<T, AKC, BKC, BM, BN, WM, WN, KB, ST, OCC, true>;
+    static std::atomic<uint64_t> done;
+    allow_lds((const void*)fn, lds, done);
+    hipLaunchKernelGGL(fn, grid, dim3(256), lds, s, a, e);
   } else {
-    const auto fn = &k_dense<T, AKC, BKC, BM, BN, WM, WN, false>;
-    dgprf::set_lds_limit((const void*)fn, lds);
-    hipLaunchKernelGGL(fn, grid, dim3(NT), lds, s, a, e);
+    const auto fn = &k_dense<T, AKC, BKC, BM, BN, WM, WN, KB, ST, OCC, false>;
+    static std::atomic<uint64_t> done;
+    allow_lds((const void*)fn, lds, done);
+    hipLaunchKernelGGL(fn, grid, dim3(256), lds, s, a, e);
   }
   return hipGetLastError();
 }
 
 template <class T, bool AKC, bool BKC>
 hipError_t launch_layout(int tile, const GemmArgs& a, const EpiDev& e, hipStream_t s) {
-  if (tile == TILE_256) return launch_tile<T, AKC, BKC, 256, 256, 128, 64>(a, e, s);
-  if (tile == TILE_128) return launch_tile<T, AKC, BKC, 128, 128, 64, 64>(a, e, s);
-  return launch_tile<T, AKC, BKC, 32, 128, 32, 32>(a, e, s);
+  if constexpr (sizeof(T) == 2) {
+    if (tile == TILE_256) return launch_tile<T, AKC, BKC, 256, 256, 128, 128, 128, 2, 1>(a, e, s);
+    if (tile == TILE_256N) return launch_tile<T, AKC, BKC, 256, 128, 128, 64, 64, 3, 2>(a, e, s);
+  }
+  if (tile == TILE_128) return launch_tile<T, AKC, BKC, 128, 128, 64, 64, 64, 4, 2>(a, e, s);
+  if (tile == TILE_64) return launch_tile<T, AKC, BKC, 64, 64, 32, 32, 128, 2, 4>(a, e, s);
+  return launch_tile<T, AKC, BKC, 32, 128, 32, 32, 128, 2, 4>(a, e, s);
 }
 
 template <class T>

@@ -12,17 +12,20 @@
 //                          utils.py:10-44, models/regression_model.py:33-50,
 //                          experiments/utils_training.py:63-65
 //   dgprf::lse_finalize    experiments/utils_training.py:79-85
-//   dgprf::linear, linear_backward, dropout   the dense operators (include/dgprf.h): every size,
-//                          type and stride is checked here, before anything is enqueued
+//   dgprf::linear, dropout the dense operators (include/dgprf.h), differentiable: every size, type and
+//                          stride is checked here, before anything is enqueued
 #include <cmath>
 #include <cstring>
 #include <string>
 #include <vector>
 
+#include <ATen/ops/add.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
 #include "../../include/dgprf.h"
@@ -237,152 +240,244 @@ std::tuple<Tensor, Tensor> lse_finalize(const Tensor& m, const Tensor& s, const 
 }
 
 // ---------------------------------------------------------------- dense operators
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
 int32_t dense_type(const Tensor& t, const char* what) {
-  TORCH_CHECK(t.is_cuda(), "dgprf: ", what, " must be a HIP tensor");
   if (t.scalar_type() == at::kFloat) return DGPRF_F32;
   if (t.scalar_type() == at::kHalf) return DGPRF_F16;
   TORCH_CHECK_TYPE(t.scalar_type() == at::kBFloat16, "dgprf: ", what,
                    " must be float32, float16 or bfloat16, got ", t.scalar_type());
   return DGPRF_BF16;
 }
-// same element type and device as x; [rows, cols] with unit stride within a row
-void dense_like(const Tensor& t, const Tensor& x, int64_t rows, int64_t cols, const char* what) {
+// same element type and device as x
+void dense_like(const Tensor& t, const Tensor& x, const char* what) {
   TORCH_CHECK_TYPE(t.scalar_type() == x.scalar_type(), "dgprf: ", what, " is ", t.scalar_type(), ", x is ",
                    x.scalar_type(), " (one type for a call)");
   TORCH_CHECK_VALUE(t.device() == x.device(), "dgprf: ", what, " is on ", t.device(), ", x is on ", x.device());
-  TORCH_CHECK_VALUE(t.dim() == 2 && t.size(0) == rows && t.size(1) == cols, "dgprf: ", what, " must be [", rows,
-                    ", ", cols, "], got ", t.sizes());
-  TORCH_CHECK_VALUE(cols <= 1 || t.stride(1) == 1, "dgprf: ", what, " must have unit stride within a row");
+}
+bool given(const OptT& t) { return t.has_value() && t->defined(); }
+
+// [..., n] as a matrix that the kernels can read: unit stride within a row, rows apart by 0 or by n and
+// more.  A view where the strides allow one.
+Tensor rows_of(const Tensor& t, int64_t n) {
+  const Tensor m = t.dim() == 2 ? t : t.reshape({-1, n});
+  const bool ok = (n <= 1 || m.stride(1) == 1) &&
+                  (m.size(0) <= 1 || m.stride(0) == 0 || m.stride(0) >= n);
+  return ok ? m : m.contiguous();
 }
 int64_t row_stride(const Tensor& t) { return t.size(0) <= 1 ? t.size(1) : t.stride(0); }
+// the same where rows may not share memory
+Tensor apart(const Tensor& t) { return t.size(0) > 1 && t.stride(0) < t.size(1) ? t.contiguous() : t; }
 
-void check_drop(int64_t thr, const Tensor& x, const OptT& step) {
-  TORCH_CHECK_VALUE(thr >= 0 && thr <= 65536, "dgprf: dropout threshold must be in [0, 65536], got ", thr);
-  if (step.has_value() && step->defined())
-    TORCH_CHECK_VALUE(step->device() == x.device() && step->scalar_type() == at::kLong && step->numel() >= 1,
+struct Drop {
+  int64_t thr, seed, sub;
+  Tensor step;  // undefined: none
+  Drop(int64_t thr_, int64_t seed_, int64_t sub_, const OptT& step_, const Tensor& x)
+      : thr(thr_), seed(seed_), sub(sub_) {
+    TORCH_CHECK_VALUE(thr >= 0 && thr <= 65536, "dgprf: dropout threshold must be in [0, 65536], got ", thr);
+    if (!given(step_)) return;
+    TORCH_CHECK_VALUE(step_->device() == x.device() && step_->scalar_type() == at::kLong && step_->numel() >= 1,
                       "dgprf: step must be an int64 tensor on the device of x");
-}
-const int64_t* step_of(const OptT& step) {
-  return step.has_value() && step->defined() ? step->data_ptr<int64_t>() : nullptr;
-}
-const void* ptr_of(const OptT& t) { return t.has_value() && t->defined() ? t->data_ptr() : nullptr; }
+    if (thr) step = *step_;
+  }
+  const int64_t* ptr() const { return step.defined() ? step.data_ptr<int64_t>() : nullptr; }
+};
 
-// (y [m, n], aux: what backward needs of z, or empty)
-std::tuple<Tensor, Tensor> linear(const Tensor& x, const Tensor& w, const OptT& bias, int64_t act,
-                                  const OptT& res, int64_t thr, int64_t seed, int64_t sub, const OptT& step,
-                                  bool save) {
+Tensor scratch_of(int64_t bytes, const Tensor& x) {
+  return bytes ? at::empty({bytes}, x.options().dtype(at::kByte)) : Tensor();
+}
+
+// y [m, n]; aux: if not null, receives what backward needs of z (nothing for no activation)
+Tensor linear_call(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& res, int64_t act,
+                   const Drop& drop, Tensor* aux) {
   dgprf_linear_t a;
   std::memset(&a, 0, sizeof(a));
+  const c10::DeviceGuard guard(x.device());
   a.dtype = dense_type(x, "x");
-  TORCH_CHECK_VALUE(x.dim() == 2 && w.dim() == 2, "dgprf: x and weight must be matrices");
+  a.act = (int32_t)act;
   a.m = x.size(0);
   a.k = x.size(1);
   a.n = w.size(1);
-  dense_like(x, x, a.m, a.k, "x");
-  dense_like(w, x, a.k, a.n, "weight");
-  if (bias.has_value() && bias->defined()) {
-    TORCH_CHECK_VALUE(bias->dim() == 1, "dgprf: bias must be [", a.n, "], got ", bias->sizes());
-    TORCH_CHECK_VALUE(bias->stride(0) == 1 || bias->size(0) <= 1, "dgprf: bias must be contiguous");
-    dense_like(bias->unsqueeze(0), x, 1, a.n, "bias");
-  }
-  if (res.has_value() && res->defined()) {
-    dense_like(*res, x, a.m, a.n, "residual");
-    a.ldr = row_stride(*res);
-  }
-  check_drop(thr, x, step);
-  const c10::DeviceGuard guard(x.device());
-  a.act = (int32_t)act;
   a.ldx = row_stride(x);
   a.ldw = row_stride(w);
   a.x = x.data_ptr();
   a.w = w.data_ptr();
-  a.bias = ptr_of(bias);
-  a.res = ptr_of(res);
-  a.drop_thr = (int32_t)thr;
-  a.seed = (uint64_t)seed;
-  a.sub = (uint64_t)sub;
-  a.step = step_of(step);
+  if (bias.defined()) a.bias = bias.data_ptr();
+  if (res.defined()) {
+    a.res = res.data_ptr();
+    a.ldr = row_stride(res);
+  }
+  a.drop_thr = (int32_t)drop.thr;
+  a.seed = (uint64_t)drop.seed;
+  a.sub = (uint64_t)drop.sub;
+  a.step = drop.ptr();
   int64_t need = 0;
   check_rc(dgprf_linear_scratch(&a, &need), "dgprf_linear_forward");
   Tensor y = at::empty({a.m, a.n}, x.options());
-  const bool keep = save && act != DGPRF_ACT_NONE;
-  Tensor aux = at::empty({keep ? a.m : 0, keep ? (a.n + 7) / 8 * 8 : 0}, x.options());
   a.y = y.data_ptr();
-  a.aux = keep ? aux.data_ptr() : nullptr;
-  Tensor scratch;
-  if (need) scratch = at::empty({need}, x.options().dtype(at::kByte));
-  check_rc(dgprf_linear_forward(&a, need ? scratch.data_ptr() : nullptr, need, stream()),
-           "dgprf_linear_forward");
-  return {y, aux};
-}
-
-// gradients of x, weight and bias (those asked for; the others are empty)
-std::tuple<Tensor, Tensor, Tensor> linear_backward(const Tensor& dy, const Tensor& x, const Tensor& w,
-                                                   const OptT& aux, int64_t act, int64_t thr, int64_t seed,
-                                                   int64_t sub, const OptT& step, bool want_x, bool want_w,
-                                                   bool want_b) {
-  dgprf_linear_grad_t a;
-  std::memset(&a, 0, sizeof(a));
-  a.dtype = dense_type(x, "x");
-  TORCH_CHECK_VALUE(x.dim() == 2 && w.dim() == 2, "dgprf: x and weight must be matrices");
-  a.m = x.size(0);
-  a.k = x.size(1);
-  a.n = w.size(1);
-  dense_like(x, x, a.m, a.k, "x");
-  dense_like(w, x, a.k, a.n, "weight");
-  dense_like(dy, x, a.m, a.n, "dy");
-  if (act != DGPRF_ACT_NONE) {
-    TORCH_CHECK_VALUE(aux.has_value() && aux->defined(), "dgprf: the saved tensor of the forward pass is missing");
-    dense_like(*aux, x, a.m, (a.n + 7) / 8 * 8, "aux");
-    TORCH_CHECK_VALUE(aux->is_contiguous(), "dgprf: aux must be contiguous");
+  if (aux && act != DGPRF_ACT_NONE) {
+    *aux = at::empty({a.m, (a.n + 7) / 8 * 8}, x.options());
     a.aux = aux->data_ptr();
   }
-  check_drop(thr, x, step);
-  const c10::DeviceGuard guard(x.device());
-  a.act = (int32_t)act;
-  a.ldx = row_stride(x);
-  a.ldw = row_stride(w);
-  a.lddy = row_stride(dy);
-  a.x = x.data_ptr();
-  a.w = w.data_ptr();
-  a.dy = dy.data_ptr();
-  a.drop_thr = (int32_t)thr;
-  a.seed = (uint64_t)seed;
-  a.sub = (uint64_t)sub;
-  a.step = step_of(step);
-  const auto none = std::vector<int64_t>{0};
-  Tensor dx = want_x ? at::empty({a.m, a.k}, x.options()) : at::empty(none, x.options());
-  Tensor dw = want_w ? at::empty({a.k, a.n}, x.options()) : at::empty(none, x.options());
-  Tensor db = want_b ? at::empty({a.n}, x.options()) : at::empty(none, x.options());
-  a.dx = want_x ? dx.data_ptr() : nullptr;
-  a.dw = want_w ? dw.data_ptr() : nullptr;
-  a.db = want_b ? db.data_ptr() : nullptr;
-  int64_t need = 0;
-  check_rc(dgprf_linear_grad_scratch(&a, &need), "dgprf_linear_backward");
-  Tensor scratch;
-  if (need) scratch = at::empty({need}, x.options().dtype(at::kByte));
-  check_rc(dgprf_linear_backward(&a, need ? scratch.data_ptr() : nullptr, need, stream()),
-           "dgprf_linear_backward");
-  return {dx, dw, db};
+  const Tensor scratch = scratch_of(need, x);
+  check_rc(dgprf_linear_forward(&a, need ? scratch.data_ptr() : nullptr, need, stream()),
+           "dgprf_linear_forward");
+  return y;
 }
 
-Tensor dropout(const Tensor& x, const OptT& res, int64_t thr, int64_t seed, int64_t sub, const OptT& step) {
-  const int32_t dtype = dense_type(x, "x");
-  TORCH_CHECK_VALUE(x.dim() == 2, "dgprf: x must be [rows, n]");
-  const int64_t rows = x.size(0), n = x.size(1);
-  dense_like(x, x, rows, n, "x");
-  int64_t ldr = 0;
-  if (res.has_value() && res->defined()) {
-    dense_like(*res, x, rows, n, "residual");
-    ldr = row_stride(*res);
-  }
-  check_drop(thr, x, step);
+Tensor dropout_call(const Tensor& x, const Tensor& res, const Drop& drop) {
   const c10::DeviceGuard guard(x.device());
-  Tensor y = at::empty({rows, n}, x.options());
-  check_rc(dgprf_dropout(dtype, x.data_ptr(), rows, n, row_stride(x), ptr_of(res), ldr, (int32_t)thr,
-                         (uint64_t)seed, (uint64_t)sub, step_of(step), y.data_ptr(), stream()),
+  Tensor y = at::empty({x.size(0), x.size(1)}, x.options());
+  check_rc(dgprf_dropout(dense_type(x, "x"), x.data_ptr(), x.size(0), x.size(1), row_stride(x),
+                         res.defined() ? res.data_ptr() : nullptr, res.defined() ? row_stride(res) : 0,
+                         (int32_t)drop.thr, (uint64_t)drop.seed, (uint64_t)drop.sub, drop.ptr(), y.data_ptr(),
+                         stream()),
            "dgprf_dropout");
   return y;
+}
+
+// A gradient of these gradients would leave terms out silently: it is an error instead.
+variable_list once(variable_list grads, const char* what) {
+  if (!at::GradMode::is_enabled()) return grads;
+  const auto error = std::make_shared<torch::autograd::DelayedError>(
+      std::string("dgprf: ") + what + " has no second derivative", (int64_t)grads.size());
+  return (*error)(std::move(grads));
+}
+
+struct LinearFunction : public torch::autograd::Function<LinearFunction> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptT& bias,
+                        const OptT& res, int64_t act, int64_t thr, int64_t seed, int64_t sub, const OptT& step) {
+    const Drop drop(thr, seed, sub, step, x);
+    const bool save = x.requires_grad() || w.requires_grad() || (given(bias) && bias->requires_grad());
+    Tensor aux;
+    Tensor y = linear_call(x, w, given(bias) ? *bias : Tensor(), given(res) ? *res : Tensor(), act, drop,
+                           save ? &aux : nullptr);
+    ctx->save_for_backward({x, w, aux, drop.step});
+    ctx->saved_data["args"] = std::vector<int64_t>{act, thr, seed, sub, given(bias), given(res)};
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &w = saved[1], &aux = saved[2], &step = saved[3];
+    const auto args = ctx->saved_data["args"].toIntVector();
+    const bool bias = args[4], res = args[5];
+    const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
+    const bool want_b = bias && ctx->needs_input_grad(2), want_r = res && ctx->needs_input_grad(bias ? 3 : 2);
+    Tensor dx, dw, db;
+    if (want_x || want_w || want_b) {
+      const at::NoGradGuard no_grad;
+      const c10::DeviceGuard guard(x.device());
+      const Tensor dy = rows_of(grads[0], w.size(1));
+      dgprf_linear_grad_t a;
+      std::memset(&a, 0, sizeof(a));
+      a.dtype = dense_type(x, "x");
+      a.act = (int32_t)args[0];
+      a.m = x.size(0);
+      a.k = x.size(1);
+      a.n = w.size(1);
+      a.ldx = row_stride(x);
+      a.ldw = row_stride(w);
+      a.lddy = row_stride(dy);
+      a.x = x.data_ptr();
+      a.w = w.data_ptr();
+      a.dy = dy.data_ptr();
+      if (aux.defined()) a.aux = aux.data_ptr();
+      a.drop_thr = (int32_t)args[1];
+      a.seed = (uint64_t)args[2];
+      a.sub = (uint64_t)args[3];
+      if (step.defined()) a.step = step.data_ptr<int64_t>();
+      if (want_x) a.dx = (dx = at::empty({a.m, a.k}, x.options())).data_ptr();
+      if (want_w) a.dw = (dw = at::empty({a.k, a.n}, x.options())).data_ptr();
+      if (want_b) a.db = (db = at::empty({a.n}, x.options())).data_ptr();
+      int64_t need = 0;
+      check_rc(dgprf_linear_grad_scratch(&a, &need), "dgprf_linear_backward");
+      const Tensor scratch = scratch_of(need, x);
+      check_rc(dgprf_linear_backward(&a, need ? scratch.data_ptr() : nullptr, need, stream()),
+               "dgprf_linear_backward");
+    }
+    const Tensor none;
+    return once({dx, dw, db, want_r ? grads[0] : none, none, none, none, none, none}, "linear");
+  }
+};
+
+struct DropoutFunction : public torch::autograd::Function<DropoutFunction> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptT& res, int64_t thr, int64_t seed,
+                        int64_t sub, const OptT& step) {
+    const Drop drop(thr, seed, sub, step, x);
+    ctx->save_for_backward({drop.step});
+    ctx->saved_data["args"] = std::vector<int64_t>{thr, seed, sub, given(res)};
+    return dropout_call(x, given(res) ? *res : Tensor(), drop);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const Tensor step = ctx->get_saved_variables()[0];
+    const auto args = ctx->saved_data["args"].toIntVector();
+    Tensor dx;
+    if (ctx->needs_input_grad(0)) {
+      const at::NoGradGuard no_grad;
+      const Tensor dy = rows_of(grads[0], grads[0].size(1));
+      dx = dropout_call(dy, Tensor(), Drop(args[0], args[1], args[2], step, dy));
+    }
+    const Tensor none;
+    return once({dx, args[3] && ctx->needs_input_grad(1) ? grads[0] : none, none, none, none, none}, "dropout");
+  }
+};
+
+bool tracks(const OptT& t) { return given(t) && t->requires_grad(); }
+constexpr const char* kNoCpu = ": the dense operators need a HIP device (there is no CPU fallback)";
+
+Tensor linear(const Tensor& x, const Tensor& weight, const OptT& bias, int64_t act, const OptT& residual,
+              int64_t thr, int64_t seed, int64_t sub, const OptT& step) {
+  dense_type(x, "x");
+  TORCH_CHECK(x.is_cuda(), "dgprf: x is on ", x.device(), kNoCpu);
+  dense_like(weight, x, "weight");
+  TORCH_CHECK_VALUE(x.dim() >= 1 && weight.dim() == 2 && x.size(-1) == weight.size(0),
+                    "dgprf: x [..., k] and weight [k, n] do not fit: ", x.sizes(), ", ", weight.sizes());
+  const int64_t k = weight.size(0), n = weight.size(1);
+  TORCH_CHECK_VALUE(k >= 1 && n >= 1, "dgprf: weight must not be empty, got ", weight.sizes());
+  auto shape = x.sizes().vec();
+  shape.back() = n;
+  OptT b = bias, r = residual;
+  if (given(b)) {
+    dense_like(*b, x, "bias");
+    TORCH_CHECK_VALUE(b->dim() == 1 && b->size(0) == n, "dgprf: bias must be [", n, "], got ", b->sizes());
+    b = b->contiguous();
+  }
+  if (given(r)) {
+    dense_like(*r, x, "residual");
+    TORCH_CHECK_VALUE(r->sizes() == at::IntArrayRef(shape), "dgprf: residual must have the result's shape ",
+                      at::IntArrayRef(shape), ", got ", r->sizes());
+    r = rows_of(*r, n);
+  }
+  const Tensor x2 = apart(rows_of(x, k)), w = apart(rows_of(weight, n));
+  Tensor y;
+  if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || tracks(bias) || tracks(residual)))
+    y = LinearFunction::apply(x2, w, b, r, act, thr, seed, sub, step);
+  else
+    y = linear_call(x2, w, given(b) ? *b : Tensor(), given(r) ? *r : Tensor(), act,
+                    Drop(thr, seed, sub, step, x), nullptr);
+  return x.dim() == 2 ? y : y.view(shape);
+}
+
+Tensor dropout(const Tensor& x, const OptT& residual, int64_t thr, int64_t seed, int64_t sub, const OptT& step) {
+  dense_type(x, "x");
+  TORCH_CHECK(x.is_cuda(), "dgprf: x is on ", x.device(), kNoCpu);
+  TORCH_CHECK_VALUE(x.dim() >= 1, "dgprf: x must have at least one dimension");
+  const int64_t n = x.size(-1);
+  OptT r = residual;
+  if (given(r)) {
+    dense_like(*r, x, "residual");
+    TORCH_CHECK_VALUE(r->sizes() == x.sizes(), "dgprf: residual must have x's shape ", x.sizes(), ", got ", r->sizes());
+  }
+  if (x.numel() == 0) return given(r) ? at::add(x, *r) : x.clone();
+  if (given(r)) r = rows_of(*r, n);
+  const Tensor x2 = rows_of(x, n);
+  Tensor y;
+  if (at::GradMode::is_enabled() && (x.requires_grad() || tracks(residual)))
+    y = DropoutFunction::apply(x2, r, thr, seed, sub, step);
+  else
+    y = dropout_call(x2, given(r) ? *r : Tensor(), Drop(thr, seed, sub, step, x));
+  return x.dim() == 2 ? y : y.view(x.sizes());
 }
 
 }  // namespace
@@ -411,10 +506,10 @@ TORCH_LIBRARY(dgprf, m) {
   m.def("lse_finalize(Tensor m, Tensor s, Tensor? e, float s_total, float y_std, bool lse_out) "
         "-> (Tensor, Tensor)");
   m.def("linear(Tensor x, Tensor weight, Tensor? bias, int act, Tensor? residual, int drop_thr, int seed, "
-        "int sub, Tensor? step, bool save) -> (Tensor, Tensor)");
-  m.def("linear_backward(Tensor dy, Tensor x, Tensor weight, Tensor? aux, int act, int drop_thr, int seed, "
-        "int sub, Tensor? step, bool want_x, bool want_w, bool want_b) -> (Tensor, Tensor, Tensor)");
-  m.def("dropout(Tensor x, Tensor? residual, int drop_thr, int seed, int sub, Tensor? step) -> Tensor");
+        "int sub, Tensor? step) -> Tensor",
+        &linear);
+  m.def("dropout(Tensor x, Tensor? residual, int drop_thr, int seed, int sub, Tensor? step) -> Tensor",
+        &dropout);
 }
 
 TORCH_LIBRARY_IMPL(dgprf, CUDA, m) {
@@ -423,7 +518,4 @@ TORCH_LIBRARY_IMPL(dgprf, CUDA, m) {
   m.impl("forward", &forward);
   m.impl("forward_samples", &forward_samples);
   m.impl("lse_finalize", &lse_finalize);
-  m.impl("linear", &linear);
-  m.impl("linear_backward", &linear_backward);
-  m.impl("dropout", &dropout);
 }

@@ -96,8 +96,10 @@ def test_python_refusals():
         dgprf.dropout(x, 0.5)
     with pytest.raises(TypeError):
         dgprf.linear(x.double(), w)
-    with pytest.raises(TypeError):
+    with pytest.raises((TypeError, RuntimeError)):
         dgprf.linear([[1.0]], w)
+    with pytest.raises(ValueError, match="activation"):
+        dgprf.linear(x, w, activation="swish")
     for p in (-0.1, 1.1, float("nan")):
         with pytest.raises(ValueError):
             dgprf.dense.drop_threshold(p)
