@@ -282,21 +282,40 @@ struct Shape {
 constexpr int kRowsMax = 8;  // rows the streaming kernel takes
 constexpr int64_t kMaxWidth = 1 << 20;  // a tile's rows stay within a buffer descriptor's range
 
-// Tile and parts of K for an I x J result.
+// Tile and parts of K for an I x J result: the pair with the least estimated time.  A CU that gets c
+// workgroups takes  fixed + c (out + rate K / parts)  microseconds (K in units of 1024); joining P
+// parts costs a launch and P I J 8 bytes of traffic at 5.5 TB/s.  The three numbers of a tile come from
+// runs with one to four workgroups per CU at K = 512 .. 8192 (4096 x 2048 x 4096 in bf16: 60 us with
+// 256 x 256 tiles, 68 with 256 x 128, 76 with 128 x 128; 2048 x 2048 x 2048: 47, 32, 23, and 30 with
+// 64 x 64; 64 x 4096 x 4096: 12.4 with 32 x 128 and four parts, 19 with one).
+struct TileCost {
+  float fixed, out, rate;
+};
+constexpr TileCost kCost16[TILES] = {{3.f, 12.f, 22.5f}, {9.f, 1.f, 14.4f}, {5.f, 0.5f, 9.2f}, {4.5f, 0.5f, 3.3f}, {4.f, 0.5f, 3.4f}};
+// fp32: 65 us of 4096 multiply-adds a clock; the 256-wide tiles' accumulators and fragments do not fit
+constexpr TileCost kCost32[TILES] = {{0, 0, 0}, {0, 0, 0}, {5.f, 1.f, 59.f}, {5.f, 0.5f, 17.f}, {5.f, 0.5f, 17.5f}};
+
 Shape shape_of(int64_t I, int64_t J, int64_t K, int es) {
-  Shape s;
-  const int64_t big = cdiv(I, 256) * cdiv(J, 256);
-  s.tile = es == 4 ? TILE_64 : I <= 32 ? TILE_32 : big >= 160 ? TILE_256 : TILE_128;
-  const TileShape ts = kTiles[s.tile];
-  s.n_mt = (int)cdiv(I, ts.bm);
-  s.n_nt = (int)cdiv(J, ts.bn);
-  s.stages = (int)cdiv(K * es, ts.kb);
-  const int64_t tiles = (int64_t)s.n_mt * s.n_nt;
-  int64_t want = tiles < 256 ? cdiv(512, tiles) : 1;
-  want = std::min<int64_t>({want, std::max(1, s.stages * ts.kb / 512), 32});
-  s.stages_split = (int)cdiv(s.stages, want);
-  s.splits = (int)cdiv(s.stages, s.stages_split);
-  return s;
+  Shape best{};
+  float least = INFINITY;
+  for (int tile = es == 4 ? TILE_128 : TILE_256; tile < TILES; ++tile) {
+    const TileShape ts = kTiles[tile];
+    const TileCost tc = es == 4 ? kCost32[tile] : kCost16[tile];
+    const int64_t mt = cdiv(I, ts.bm), nt = cdiv(J, ts.bn), stages = cdiv(K * es, ts.kb);
+    if (mt * nt >= (int64_t)1 << 26) continue;  // workgroups of a launch, times 32 parts at most
+    for (int64_t want = 1; want <= 32; want *= 2) {
+      if (want > 1 && stages < 4 * want) break;
+      const int64_t per = cdiv(stages, want), parts = cdiv(stages, per);
+      const float k = (float)per * ts.kb / es / 1024.f, rounds = (float)cdiv(mt * nt * parts, 256);
+      float t = tc.fixed + rounds * (tc.out + tc.rate * k);
+      if (parts > 1) t += 3.f + (float)parts * I * J * 8.f / 5.5e6f;
+      if (t < least) {
+        least = t;
+        best = Shape{tile, (int)mt, (int)nt, (int)parts, (int)stages, (int)per};
+      }
+    }
+  }
+  return best;
 }
 int64_t part_bytes(const Shape& s, int64_t I, int64_t J) {
   return s.splits > 1 ? up((int64_t)s.splits * I * up(J, 8) * 4, 256) : 0;

@@ -559,8 +559,8 @@ hipError_t launch_layout(int tile, const GemmArgs& a, const EpiDev& e, hipStream
     if (tile == TILE_256N) return launch_tile<T, AKC, BKC, 256, 128, 128, 64, 64, 3, 2>(a, e, s);
   }
   if (tile == TILE_128) return launch_tile<T, AKC, BKC, 128, 128, 64, 64, 64, 4, 2>(a, e, s);
-  if (tile == TILE_64) return launch_tile<T, AKC, BKC, 64, 64, 32, 32, 128, 2, 4>(a, e, s);
-  return launch_tile<T, AKC, BKC, 32, 128, 32, 32, 128, 2, 4>(a, e, s);
+  if (tile == TILE_64) return launch_tile<T, AKC, BKC, 64, 64, 32, 32, 128, 3, 3>(a, e, s);
+  return launch_tile<T, AKC, BKC, 32, 128, 32, 32, 128, 4, 2>(a, e, s);
 }
 
 template <class T>
