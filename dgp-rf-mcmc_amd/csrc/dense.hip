@@ -13,21 +13,29 @@ inline int64_t up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 inline int64_t cdiv(int64_t x, int64_t m) { return (x + m - 1) / m; }
 
 // ---------------------------------------------------------------- packing
-// Rows of `cols` elements at any stride and alignment to rows of ldo, zero-padded: the tiled product
-// reads 16 bytes at a time.
+// Rows of `cols` elements at any stride and alignment to rows of a multiple of eight, zero-padded: the
+// tiled product reads 16 bytes at a time.  Two matrices a launch, so that a product with two odd operands
+// pays one.
+struct PackDev {
+  const void* in;
+  void* out;  // null: no matrix
+  int64_t ld;
+  int32_t rows, cols;
+  __host__ __device__ int per() const { return (cols + 7) >> 3; }
+  __host__ __device__ int64_t blocks() const { return out ? ((int64_t)rows * per() + 255) / 256 : 0; }
+};
 template <class T>
-__global__ __launch_bounds__(256) void k_pack(const T* __restrict__ in, int64_t ld, int rows, int cols,
-                                              T* __restrict__ out, int ldo) {
-  const int per = ldo >> 3;  // ldo % 8 == 0
-  const int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (q >= (int64_t)rows * per) return;
+__global__ __launch_bounds__(256) void k_pack(const PackDev a, const PackDev b) {
+  const int64_t na = a.blocks();
+  const bool first = blockIdx.x < na;
+  const PackDev p = first ? a : b;
+  const int per = p.per();
+  const int64_t q = (int64_t)(first ? blockIdx.x : blockIdx.x - na) * 256 + threadIdx.x;
+  if (q >= (int64_t)p.rows * per) return;
   const int64_t row = q / per;
   const int col = (int)(q - row * per) * 8;
-  const T* p = in + row * ld;
-  typename Vec<T>::v8 v;
-#pragma unroll
-  for (int c = 0; c < 8; ++c) v[c] = col + c < cols ? p[col + c] : (T)0.f;
-  *reinterpret_cast<typename Vec<T>::v8*>(out + row * ldo + col) = v;
+  const F8 v = load8((const T*)p.in + row * p.ld, col, p.cols);
+  store8_whole((T*)p.out + row * (per * 8) + col, v);
 }
 
 // ---------------------------------------------------------------- joining the parts of K
@@ -66,30 +74,45 @@ __global__ __launch_bounds__(256) void k_join(const float* __restrict__ part, in
     v.hi += sums[w][1][lane];
   }
   F8 b{f4zero(), f4zero()};
-  if (e.bias) b = load8((const T*)e.bias, col, n, false);
+  if (e.bias) b = load8((const T*)e.bias, col, n);
   const uint64_t sub = e.drop.thr ? drop_sub(e.drop) : 0;
   with_act(e.act, [&](auto act) { v = value_of<T, decltype(act)::value>(e, row, col, sub, v, b); });
   if (e.res) {
-    const F8 r = load8((const T*)e.res + row * e.ldr, col, n, e.vec_r);
+    const F8 r = load8((const T*)e.res + row * e.ldr, col, n);
     v.lo += r.lo;
     v.hi += r.hi;
   }
-  store8((T*)e.y + row * e.ldy, col, n, e.vec_y, v);
+  store8((T*)e.y + row * e.ldy, col, n, v);
 }
 
 // ---------------------------------------------------------------- few rows
-// z = x W for up to MR rows: W is read once, at memory speed, by many workgroups, and each product is
-// a plain multiply-add (2 MR operations a weight; the matrix instructions would pad MR to 16).  A
+// z = x W for one row, or two of a long K: W is read once, at memory speed, by many workgroups, and each
+// product is a plain multiply-add (from three rows on the tiled product is faster: 4 x 2048 x 8192 in bf16
+// 13.2 us, 15.3 this way; 2 x 4096 x 4096 12.9 and 11.4).  A
 // workgroup takes 16 lanes' width of columns and up to 1024 k; its 16 k-lanes (4 of a wave, 4 waves)
 // take groups of four k each, whose x values are one LDS read, and their sums are added in a fixed
 // order.  Parts of K are joined by k_join.
+template <class T>
+struct Piece {  // 16 bytes of a row
+  typedef T vec __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+};
+// the first `there` elements of a piece, zeros behind them
+template <class T>
+__device__ __forceinline__ typename Piece<T>::vec load_piece(const T* p, int there) {
+  constexpr int CE = 16 / (int)sizeof(T);
+  if (there >= CE) return *reinterpret_cast<const typename Piece<T>::vec*>(p);
+  typename Piece<T>::vec v;
+#pragma unroll
+  for (int c = 0; c < CE; ++c) v[c] = c < there ? p[c] : (T)0.f;
+  return v;
+}
 constexpr int kRowsK = 1024;
-template <class T, int MR, bool VEC>
+template <class T, int MR>
 __global__ __launch_bounds__(256) void k_rows(const T* __restrict__ x, int64_t ldx,
                                               const T* __restrict__ w, int64_t ldw, int M, int K, int N,
                                               int k_part, float* __restrict__ part, int64_t ldp) {
   constexpr int CE = 16 / (int)sizeof(T), STRIP = 16 * CE;
-  typedef T vec __attribute__((ext_vector_type(CE)));
+  typedef typename Piece<T>::vec vec;
   __shared__ __attribute__((aligned(16))) float xs[MR * kRowsK];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int k0 = blockIdx.y * k_part, kn = min(k_part, K - k0), kp = (kn + 3) & ~3;
@@ -108,19 +131,9 @@ __global__ __launch_bounds__(256) void k_rows(const T* __restrict__ x, int64_t l
     const T* wp = w + (int64_t)k0 * ldw + col;
 #pragma unroll 2
     for (int k = (wave * 4 + (lane >> 4)) * 4; k < kn; k += 64) {
-      T v[4][CE];
+      vec v[4];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const T* p = wp + (int64_t)(k + r) * ldw;
-        if constexpr (VEC) {
-          const vec u = k + r < kn ? *reinterpret_cast<const vec*>(p) : (vec)(T)0.f;
-#pragma unroll
-          for (int c = 0; c < CE; ++c) v[r][c] = u[c];
-        } else {
-#pragma unroll
-          for (int c = 0; c < CE; ++c) v[r][c] = k + r < kn && col + c < N ? p[c] : (T)0.f;
-        }
-      }
+      for (int r = 0; r < 4; ++r) v[r] = k + r < kn ? load_piece<T>(wp + (int64_t)(k + r) * ldw, N - col) : (vec)(T)0.f;
 #pragma unroll
       for (int m = 0; m < MR; ++m) {
         const f4 xv = *reinterpret_cast<const f4*>(&xs[m * kRowsK + k]);
@@ -153,6 +166,75 @@ __global__ __launch_bounds__(256) void k_rows(const T* __restrict__ x, int64_t l
   }
 }
 
+// One row in one launch, for K up to kStripK: a workgroup of 16 waves takes 64 bytes of each row of W and
+// all of K, so its sums are complete and it applies the epilogue itself.  A second launch costs a row about
+// as much as the product (2048 x 4096 in bf16: 8.0 us this way, 11.7 with parts of K and k_join), but 64
+// bytes of a row at a time do not reach the memory's rate (8192 x 2048: 19 and 10.8 us): K is at most what
+// a thread has on its way at once, and W at most 8 MiB (2048 x 8192, not in a cache: 13.4 and 11.7 us).
+// Neighbouring strips go to one XCD, whose L2 their rows' lines share.
+constexpr int kStripAhead = 8, kStripK = 256 * kStripAhead;
+constexpr int64_t kStripBytes = 8 << 20;
+template <class T>
+__global__ __launch_bounds__(1024) void k_strip(const T* __restrict__ x, const T* __restrict__ w, int64_t ldw,
+                                                int K, const EpiDev e) {
+  constexpr int LPR = 4, CE = 16 / (int)sizeof(T), STRIP = LPR * CE, KL = 1024 / LPR;
+  typedef typename Piece<T>::vec vec;
+  __shared__ float xs[kStripK];
+  __shared__ __attribute__((aligned(16))) float part[16][STRIP];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, kl = tid / LPR;
+  int strip;
+  {
+    const int G = gridDim.x, b = blockIdx.x, xcd = b & 7, q = G >> 3, r = G & 7;
+    strip = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (b >> 3);
+  }
+  const int col = strip * STRIP + (tid % LPR) * CE;
+  vec v[kStripAhead];  // on the way while x is
+#pragma unroll
+  for (int u = 0; u < kStripAhead; ++u) {
+    const int k = kl + u * KL;
+    v[u] = k < K && col < e.n ? load_piece<T>(w + (int64_t)k * ldw + col, e.n - col) : (vec)(T)0.f;
+  }
+  for (int k = tid; k < K; k += 1024) xs[k] = (float)x[k];
+  __syncthreads();
+  float acc[CE];
+#pragma unroll
+  for (int c = 0; c < CE; ++c) acc[c] = 0.f;
+#pragma unroll
+  for (int u = 0; u < kStripAhead; ++u) {
+    const int k = kl + u * KL;
+    if (k < K) {
+#pragma unroll
+      for (int c = 0; c < CE; ++c) acc[c] = fmaf(xs[k], (float)v[u][c], acc[c]);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < CE; ++c) {
+    float s = acc[c];
+#pragma unroll
+    for (int d = LPR; d < 64; d *= 2) s += __shfl_xor(s, d);
+    if (lane < LPR) part[wave][lane * CE + c] = s;
+  }
+  __syncthreads();
+  const int c0 = strip * STRIP + tid * 8;
+  if (tid >= STRIP / 8 || c0 >= e.n) return;
+  F8 z{f4zero(), f4zero()}, b{f4zero(), f4zero()};
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const f4* p = reinterpret_cast<const f4*>(&part[i][tid * 8]);
+    z.lo += p[0];
+    z.hi += p[1];
+  }
+  if (e.bias) b = load8((const T*)e.bias, c0, e.n);
+  const uint64_t sub = e.drop.thr ? drop_sub(e.drop) : 0;
+  with_act(e.act, [&](auto act) { z = value_of<T, decltype(act)::value>(e, 0, c0, sub, z, b); });
+  if (e.res) {
+    const F8 r = load8((const T*)e.res, c0, e.n);
+    z.lo += r.lo;
+    z.hi += r.hi;
+  }
+  store8((T*)e.y, c0, e.n, z);
+}
+
 // ---------------------------------------------------------------- dz and its column sums
 // dz = s m dy a'(z) (rounded to the tensors' type, as the matrix instructions take it; its sums for
 // db are of the unrounded values), one thread for eight columns and `rows_part` rows; dz is null
@@ -164,7 +246,7 @@ struct DzDev {
   float* part;  // [parts][ldz] or null
   int64_t lddy, ldaux, ldz;
   int64_t M;
-  int32_t N, groups, act, vec, rows_part;
+  int32_t N, groups, act, rows_part;
   DropDev drop;
 };
 template <class T>
@@ -180,31 +262,43 @@ __global__ __launch_bounds__(256) void k_dz(const DzDev d) {
   if (gi < d.groups) {
     with_act(d.act, [&](auto act) {
       constexpr int ACT = decltype(act)::value;
-      for (int64_t m = m0 + wave; m < m1; m += 4) {
-        F8 v = load8((const T*)d.dy + m * d.lddy, col, d.N, d.vec);
-        if constexpr (ACT != DGPRF_ACT_NONE) {
-          const F8 z = load8((const T*)d.aux + m * d.ldaux, col, (int)d.ldaux, true);
+      constexpr int U = sizeof(T) == 4 ? 2 : 4;  // rows whose loads are in flight together
+      for (int64_t m = m0 + wave; m < m1; m += 4 * U) {
+        F8 g[U], z[U];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            v.lo[c] *= slope_of<T, ACT>(z.lo[c]);
-            v.hi[c] *= slope_of<T, ACT>(z.hi[c]);
-          }
+        for (int u = 0; u < U; ++u) {
+          if (m + 4 * u >= m1) continue;
+          g[u] = load8((const T*)d.dy + (m + 4 * u) * d.lddy, col, d.N);
+          if constexpr (ACT != DGPRF_ACT_NONE) z[u] = load8_whole((const T*)d.aux + (m + 4 * u) * d.ldaux + col);
         }
-        // last, so that a dropped element is 0 whatever its gradient and slope
-        if (d.drop.thr) v = drop8(v, drop_words(d.drop, sub, (uint64_t)m * (uint32_t)d.groups + (uint32_t)gi), d.drop);
-        // zeros past N: the tiled product multiplies the padding
-        if (d.dz) {
-          if (col + 8 > d.N) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (m + 4 * u >= m1) continue;
+          F8 v = g[u];
+          if constexpr (ACT != DGPRF_ACT_NONE) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-              if (col + c >= d.N) v.lo[c] = 0.f;
-              if (col + 4 + c >= d.N) v.hi[c] = 0.f;
+              v.lo[c] *= slope_of<T, ACT>(z[u].lo[c]);
+              v.hi[c] *= slope_of<T, ACT>(z[u].hi[c]);
             }
           }
-          store8((T*)d.dz + m * d.ldz, col, (int)d.ldz, true, v);
+          // last, so that a dropped element is 0 whatever its gradient and slope
+          if (d.drop.thr)
+            v = drop8(v, drop_words(d.drop, sub, (uint64_t)(m + 4 * u) * (uint32_t)d.groups + (uint32_t)gi), d.drop);
+          // zeros past N: the tiled product multiplies the padding
+          if (d.dz) {
+            if (col + 8 > d.N) {
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                if (col + c >= d.N) v.lo[c] = 0.f;
+                if (col + 4 + c >= d.N) v.hi[c] = 0.f;
+              }
+            }
+            store8_whole((T*)d.dz + (m + 4 * u) * d.ldz + col, v);
+          }
+          acc.lo += v.lo;
+          acc.hi += v.hi;
         }
-        acc.lo += v.lo;
-        acc.hi += v.hi;
       }
     });
   }
@@ -218,22 +312,24 @@ __global__ __launch_bounds__(256) void k_dz(const DzDev d) {
   }
 }
 
-// db[c] = sum of the parts: 32 columns of a workgroup, eight threads each, in a fixed order
+// db[c] = sum of the parts: 32 columns of a workgroup, 32 threads each, in a fixed order
 template <class T>
-__global__ __launch_bounds__(256) void k_db(const float* __restrict__ part, int64_t ldp, int parts, int N,
-                                            T* __restrict__ db) {
-  __shared__ float sums[8][33];
+__global__ __launch_bounds__(1024) void k_db(const float* __restrict__ part, int64_t ldp, int parts, int N,
+                                             T* __restrict__ db) {
+  __shared__ float sums[32][33];
   const int cl = threadIdx.x & 31, r = threadIdx.x >> 5, c = blockIdx.x * 32 + cl;
   float s = 0.f;
-  if (c < N)
-    for (int p = r; p < parts; p += 8) s += part[p * ldp + c];
+  if (c < N) {
+#pragma unroll 8
+    for (int p = r; p < parts; p += 32) s += part[p * ldp + c];
+  }
   sums[r][cl] = s;
   __syncthreads();
-  if (r == 0 && c < N) {
-#pragma unroll
-    for (int i = 1; i < 8; ++i) s += sums[i][cl];
-    db[c] = (T)s;
+  for (int h = 16; h > 0; h >>= 1) {
+    if (r < h) sums[r][cl] += sums[r + h][cl];
+    __syncthreads();
   }
+  if (r == 0 && c < N) db[c] = (T)sums[0][cl];
 }
 
 // ---------------------------------------------------------------- dropout
@@ -247,39 +343,37 @@ __global__ __launch_bounds__(256) void k_dropout(const T* __restrict__ x, int64_
   if (q >= total) return;
   const uint64_t sub = drop_sub(d);
   if constexpr (FLAT) {
-    F8 v = load8(x + 8 * q, 0, 8, true);
+    F8 v = load8_whole(x + 8 * q);
     if (d.thr) v = drop8(v, drop_words(d, sub, (uint64_t)q), d);
     if (res) {
-      const F8 r = load8(res + 8 * q, 0, 8, true);
+      const F8 r = load8_whole(res + 8 * q);
       v.lo += r.lo;
       v.hi += r.hi;
     }
-    store8(y + 8 * q, 0, 8, true, v);
+    store8_whole(y + 8 * q, v);
   } else {
     const int64_t row = q / groups;
     const int col = (int)(q - row * groups) * 8;
-    F8 v = load8(x + row * ldx, col, n, false);
+    F8 v = load8(x + row * ldx, col, n);
     if (d.thr) v = drop8(v, drop_words(d, sub, (uint64_t)q), d);
     if (res) {
-      const F8 r = load8(res + row * ldr, col, n, false);
+      const F8 r = load8(res + row * ldr, col, n);
       v.lo += r.lo;
       v.hi += r.hi;
     }
-    store8(y + row * (int64_t)n, col, n, false, v);
+    store8(y + row * (int64_t)n, col, n, v);
   }
 }
 
 // ---------------------------------------------------------------- choices
-int aligned(const void* p, int64_t ld, int64_t cols, int es, int bytes) {
-  return (uintptr_t)p % bytes == 0 && ld * es % bytes == 0 && cols * es % bytes == 0;
+// rows of 16-byte pieces: what the tiled product's loads to LDS read in place
+bool in_place(const void* p, int64_t ld, int64_t cols, int es) {
+  return (uintptr_t)p % 16 == 0 && ld * es % 16 == 0 && cols * es % 16 == 0;
 }
-// rows of 16-byte pieces: what the tiled product reads in place
-bool in_place(const void* p, int64_t ld, int64_t cols, int es) { return aligned(p, ld, cols, es, 16); }
 
 struct Shape {
   int tile, n_mt, n_nt, splits, stages, stages_split;
 };
-constexpr int kRowsMax = 8;  // rows the streaming kernel takes
 constexpr int64_t kMaxWidth = 1 << 20;  // a tile's rows stay within a buffer descriptor's range
 
 // Tile and parts of K for an I x J result: the pair with the least estimated time.  A CU that gets c
@@ -308,7 +402,7 @@ Shape shape_of(int64_t I, int64_t J, int64_t K, int es) {
       const int64_t per = cdiv(stages, want), parts = cdiv(stages, per);
       const float k = (float)per * ts.kb / es / 1024.f, rounds = (float)cdiv(mt * nt * parts, 256);
       float t = tc.fixed + rounds * (tc.out + tc.rate * k);
-      if (parts > 1) t += 3.f + (float)parts * I * J * 8.f / 5.5e6f;
+      if (parts > 1) t += 4.f + (float)parts * I * J * 8.f / 5.5e6f;
       if (t < least) {
         least = t;
         best = Shape{tile, (int)mt, (int)nt, (int)parts, (int)stages, (int)per};
@@ -365,14 +459,24 @@ hipError_t with_type(int dtype, F f) {
 }
 #define DENSE_T(p) typename std::remove_pointer<decltype(p)>::type
 
-hipError_t pack(int dtype, const void* in, int64_t ld, int64_t rows, int64_t cols, void* out, hipStream_t s) {
-  const int64_t ldo = up(cols, 8), q = rows * (ldo / 8);
+hipError_t pack(int dtype, const PackDev& a, const PackDev& b, hipStream_t s) {
+  const int64_t blocks = a.blocks() + b.blocks();
+  if (!blocks) return hipSuccess;
   return with_type(dtype, [&](auto* t) {
-    typedef DENSE_T(t) T;
-    hipLaunchKernelGGL((k_pack<T>), dim3((unsigned)cdiv(q, 256)), dim3(256), 0, s, (const T*)in, ld, (int)rows,
-                       (int)cols, (T*)out, (int)ldo);
+    hipLaunchKernelGGL((k_pack<DENSE_T(t)>), dim3((unsigned)blocks), dim3(256), 0, s, a, b);
     return hipGetLastError();
   });
+}
+// An operand [rows][cols] as the product reads it: in place, or a packed copy in scratch (p).  ld and
+// width become those of what is read.
+const void* operand(const void* m, int64_t* ld, int64_t rows, int64_t cols, int64_t* width, int es, Scratch& sc,
+                    PackDev* p) {
+  *p = PackDev{};
+  *width = cols;
+  if (in_place(m, *ld, cols, es)) return m;
+  *p = PackDev{m, sc.take(rows * up(cols, 8) * es), *ld, (int)rows, (int)cols};
+  *ld = *width = up(cols, 8);
+  return p->out;
 }
 
 hipError_t join(int dtype, const float* part, int64_t ldp, int parts, int64_t rows, const EpiDev& e,
@@ -386,15 +490,11 @@ hipError_t join(int dtype, const float* part, int64_t ldp, int parts, int64_t ro
 }
 
 template <class T, int MR>
-hipError_t rows_launch(const dgprf_linear_t& a, bool vec, int k_part, int parts, float* part, int64_t ldp,
+hipError_t rows_launch(const dgprf_linear_t& a, int k_part, int parts, float* part, int64_t ldp,
                        hipStream_t s) {
   const dim3 grid((unsigned)cdiv(a.n, 256 / (int)sizeof(T)), (unsigned)parts);
-  if (vec)
-    hipLaunchKernelGGL((k_rows<T, MR, true>), grid, dim3(256), 0, s, (const T*)a.x, a.ldx, (const T*)a.w, a.ldw,
-                       (int)a.m, (int)a.k, (int)a.n, k_part, part, ldp);
-  else
-    hipLaunchKernelGGL((k_rows<T, MR, false>), grid, dim3(256), 0, s, (const T*)a.x, a.ldx, (const T*)a.w, a.ldw,
-                       (int)a.m, (int)a.k, (int)a.n, k_part, part, ldp);
+  hipLaunchKernelGGL((k_rows<T, MR>), grid, dim3(256), 0, s, (const T*)a.x, a.ldx, (const T*)a.w, a.ldw, (int)a.m,
+                     (int)a.k, (int)a.n, k_part, part, ldp);
   return hipGetLastError();
 }
 
@@ -429,13 +529,12 @@ hipError_t product(int dtype, int layout, const void* A, int64_t lda, const void
   return err;
 }
 
-EpiDev epi_plain(void* y, int64_t n, int es) {
+EpiDev epi_plain(void* y, int64_t n) {
   EpiDev e{};
   e.y = y;
   e.ldy = n;
   e.n = (int)n;
   e.groups = (int)cdiv(n, 8);
-  e.vec_y = aligned(y, n, n, es, 16);
   return e;
 }
 
@@ -456,47 +555,42 @@ int check_dims(int32_t dtype, int32_t act, int64_t m, int64_t k, int64_t n, int6
 hipError_t forward(const dgprf_linear_t& a, Scratch& sc, hipStream_t st, bool run) {
   const int es = elem_size(a.dtype);
   const int64_t m = a.m, k = a.k, n = a.n;
-  EpiDev e = epi_plain(a.y, n, es);
+  EpiDev e = epi_plain(a.y, n);
   e.bias = a.bias;
   e.res = a.res;
   e.aux = a.act != DGPRF_ACT_NONE ? a.aux : nullptr;
   e.ldr = a.ldr;
   e.ldaux = up(n, 8);
   e.act = a.act;
-  e.vec_r = aligned(a.res, a.ldr, 0, es, 16);
   e.drop = drop_dev(a.drop_thr, a.seed, a.sub, a.step);
-  if (m <= kRowsMax) {
+  if (m == 1 && k <= kStripK && k * n * es <= kStripBytes) {
+    if (!run) return hipSuccess;
+    return with_type(a.dtype, [&](auto* t) {
+      typedef DENSE_T(t) T;
+      hipLaunchKernelGGL((k_strip<T>), dim3((unsigned)cdiv(n, 64 / (int)sizeof(T))), dim3(1024), 0, st,
+                         (const T*)a.x, (const T*)a.w, a.ldw, (int)k, e);
+      return hipGetLastError();
+    });
+  }
+  if (m == 1 || (m == 2 && k > kStripK)) {
     int k_part, parts;
     rows_shape(n, k, es, &k_part, &parts);
     const int64_t ldp = up(n, 8);
     float* part = (float*)sc.take((int64_t)parts * m * ldp * 4);
     if (!run) return hipSuccess;
-    const bool vec = in_place(a.w, a.ldw, n, es);
     hipError_t err = with_type(a.dtype, [&](auto* t) {
       typedef DENSE_T(t) T;
-      if (m == 1) return rows_launch<T, 1>(a, vec, k_part, parts, part, ldp, st);
-      if (m == 2) return rows_launch<T, 2>(a, vec, k_part, parts, part, ldp, st);
-      if (m <= 4) return rows_launch<T, 4>(a, vec, k_part, parts, part, ldp, st);
-      return rows_launch<T, 8>(a, vec, k_part, parts, part, ldp, st);
+      if (m == 1) return rows_launch<T, 1>(a, k_part, parts, part, ldp, st);
+      return rows_launch<T, 2>(a, k_part, parts, part, ldp, st);
     });
     return err == hipSuccess ? join(a.dtype, part, ldp, parts, m, e, st) : err;
   }
-  const void *x = a.x, *w = a.w;
-  int64_t ldx = a.ldx, ldw = a.ldw, ka = k, nb = n;
-  if (!in_place(x, ldx, k, es)) {
-    ldx = ka = up(k, 8);
-    void* p = sc.take(m * ldx * es);
-    if (run)
-      if (hipError_t err = pack(a.dtype, x, a.ldx, m, k, p, st)) return err;
-    x = p;
-  }
-  if (!in_place(w, ldw, n, es)) {
-    ldw = nb = up(n, 8);
-    void* p = sc.take(k * ldw * es);
-    if (run)
-      if (hipError_t err = pack(a.dtype, w, a.ldw, k, n, p, st)) return err;
-    w = p;
-  }
+  int64_t ldx = a.ldx, ldw = a.ldw, ka, nb;
+  PackDev px, pw;
+  const void* x = operand(a.x, &ldx, m, k, &ka, es, sc, &px);
+  const void* w = operand(a.w, &ldw, k, n, &nb, es, sc, &pw);
+  if (run)
+    if (hipError_t err = pack(a.dtype, px, pw, st)) return err;
   return product(a.dtype, LAYOUT_NN, x, ldx, w, ldw, m, n, 0, nb, ka, k, e, sc, st, run);
 }
 
@@ -524,10 +618,10 @@ hipError_t backward(const dgprf_linear_grad_t& a, Scratch& sc, hipStream_t st, b
     d.N = (int)n;
     d.groups = (int)cdiv(n, 8);
     d.act = a.act;
-    d.vec = aligned(a.dy, a.lddy, 0, es, 16);
     d.drop = drop_dev(a.drop_thr, a.seed, a.sub, a.step);
     const int64_t strips = cdiv(d.groups, 64);
-    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(cdiv(2048, strips), cdiv(m, 16)));
+    // enough workgroups to fill the memory system, and 16 rows (four a wave) in each where there are many
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(cdiv(1024, strips), cdiv(m, 16)));
     d.rows_part = (int)up(cdiv(m, want), 4);
     const int64_t parts = cdiv(m, d.rows_part);
     if (a.db) d.part = (float*)sc.take(parts * d.ldz * 4);
@@ -537,7 +631,7 @@ hipError_t backward(const dgprf_linear_grad_t& a, Scratch& sc, hipStream_t st, b
         hipLaunchKernelGGL((k_dz<T>), dim3((unsigned)strips, (unsigned)parts), dim3(256), 0, st, d);
         hipError_t er = hipGetLastError();
         if (er == hipSuccess && a.db) {
-          hipLaunchKernelGGL((k_db<T>), dim3((unsigned)cdiv(n, 32)), dim3(256), 0, st, d.part, d.ldz, (int)parts,
+          hipLaunchKernelGGL((k_db<T>), dim3((unsigned)cdiv(n, 32)), dim3(1024), 0, st, d.part, d.ldz, (int)parts,
                              (int)n, (T*)a.db);
           er = hipGetLastError();
         }
@@ -546,29 +640,17 @@ hipError_t backward(const dgprf_linear_grad_t& a, Scratch& sc, hipStream_t st, b
       if (err != hipSuccess) return err;
     }
   }
+  int64_t ldx = a.ldx, ldw = a.ldw, ka = k, nb = n;
+  PackDev px{}, pw{};
+  const void* w = a.dx ? operand(a.w, &ldw, k, n, &nb, es, sc, &pw) : nullptr;
+  const void* x = a.dw ? operand(a.x, &ldx, m, k, &ka, es, sc, &px) : nullptr;
+  if (run && (err = pack(a.dtype, pw, px, st)) != hipSuccess) return err;
   if (a.dx) {  // [m][k] = dz [m][n] (W [k][n])^T
-    const void* w = a.w;
-    int64_t ldw = a.ldw, nb = n;
-    if (!in_place(w, ldw, n, es)) {
-      ldw = nb = up(n, 8);
-      void* p = sc.take(k * ldw * es);
-      if (run && (err = pack(a.dtype, w, a.ldw, k, n, p, st)) != hipSuccess) return err;
-      w = p;
-    }
-    err = product(a.dtype, LAYOUT_NT, dz, lddz, w, ldw, m, k, 0, 0, na, nb, epi_plain(a.dx, k, es), sc, st, run);
+    err = product(a.dtype, LAYOUT_NT, dz, lddz, w, ldw, m, k, 0, 0, na, nb, epi_plain(a.dx, k), sc, st, run);
     if (err != hipSuccess) return err;
   }
-  if (a.dw) {  // [k][n] = (x [m][k])^T dz [m][n]
-    const void* x = a.x;
-    int64_t ldx = a.ldx, ka = k;
-    if (!in_place(x, ldx, k, es)) {
-      ldx = ka = up(k, 8);
-      void* p = sc.take(m * ldx * es);
-      if (run && (err = pack(a.dtype, x, a.ldx, m, k, p, st)) != hipSuccess) return err;
-      x = p;
-    }
-    err = product(a.dtype, LAYOUT_TN, x, ldx, dz, lddz, k, n, ka, na, m, m, epi_plain(a.dw, n, es), sc, st, run);
-  }
+  if (a.dw)  // [k][n] = (x [m][k])^T dz [m][n]
+    err = product(a.dtype, LAYOUT_TN, x, ldx, dz, lddz, k, n, ka, na, m, m, epi_plain(a.dw, n), sc, st, run);
   return err;
 }
 
@@ -667,8 +749,7 @@ int dgprf_dropout(int32_t dtype, const void* x, int64_t rows, int64_t n, int64_t
   const int64_t groups = cdiv(n, 8);
   if (rows > ((int64_t)1 << 39) / groups) return DGPRF_E_SHAPE;
   const int64_t total = rows * groups;
-  const bool flat = n % 8 == 0 && (rows == 1 || ldx == n) && (uintptr_t)x % 16 == 0 &&
-                    (uintptr_t)y % 16 == 0 && (!res || ((rows == 1 || ldr == n) && (uintptr_t)res % 16 == 0));
+  const bool flat = n % 8 == 0 && (rows == 1 || (ldx == n && (!res || ldr == n)));
   const DropDev d = drop_dev(drop_thr, seed, sub, step);
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   return hip_rc(with_type(dtype, [&](auto* t) {

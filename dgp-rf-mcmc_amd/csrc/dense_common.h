@@ -20,8 +20,12 @@ typedef uint32_t u32v4_t __attribute__((ext_vector_type(4)));
 
 template <class T>
 struct Vec {
-  typedef T v4 __attribute__((ext_vector_type(4)));
   typedef T v8 __attribute__((ext_vector_type(8)));
+  // 16 bytes at any element (unaligned accesses are on for this platform's processes): rows of an odd
+  // length are read and written as fast as others, where element by element a 16-bit access costs its
+  // wave some hundred clocks (1777 x 1008 x 2049 in bf16 with a residual: 43 us, 19 with n = 2048)
+  typedef T any4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  typedef T any8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
 };
 
 inline int elem_size(int dtype) { return dtype == DGPRF_F32 ? 4 : 2; }
@@ -167,7 +171,6 @@ struct EpiDev {
   int64_t ldr, ldy, ldaux;
   int32_t n, act;
   int32_t groups;    // ceil(n / 8)
-  int32_t vec_y, vec_r;  // rows of y / res allow 16-byte accesses
   DropDev drop;
 };
 
@@ -192,13 +195,13 @@ struct F8 {
   f4 lo, hi;
 };
 template <class T>
-__device__ __forceinline__ F8 load8_whole(const T* p) {  // 16-byte aligned
+__device__ __forceinline__ F8 load8_whole(const T* p) {
   F8 v;
   if constexpr (sizeof(T) == 4) {
-    v.lo = *reinterpret_cast<const f4*>(p);
-    v.hi = *reinterpret_cast<const f4*>(p + 4);
+    v.lo = *reinterpret_cast<const typename Vec<T>::any4*>(p);
+    v.hi = *reinterpret_cast<const typename Vec<T>::any4*>(p + 4);
   } else {
-    const typename Vec<T>::v8 x = *reinterpret_cast<const typename Vec<T>::v8*>(p);
+    const typename Vec<T>::any8 x = *reinterpret_cast<const typename Vec<T>::any8*>(p);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       v.lo[c] = (float)x[c];
@@ -208,32 +211,32 @@ __device__ __forceinline__ F8 load8_whole(const T* p) {  // 16-byte aligned
   return v;
 }
 template <class T>
-__device__ __forceinline__ void store8_whole(T* p, const F8& v) {  // 16-byte aligned
+__device__ __forceinline__ void store8_whole(T* p, const F8& v) {
   if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<f4*>(p) = v.lo;
-    *reinterpret_cast<f4*>(p + 4) = v.hi;
+    *reinterpret_cast<typename Vec<T>::any4*>(p) = v.lo;
+    *reinterpret_cast<typename Vec<T>::any4*>(p + 4) = v.hi;
   } else {
-    typename Vec<T>::v8 x;
+    typename Vec<T>::any8 x;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       x[c] = (T)v.lo[c];
       x[c + 4] = (T)v.hi[c];
     }
-    *reinterpret_cast<typename Vec<T>::v8*>(p) = x;
+    *reinterpret_cast<typename Vec<T>::any8*>(p) = x;
   }
 }
-// columns col .. col + 7 of a row of n; aligned: the row allows 16-byte accesses
+// columns col .. col + 7 of a row of n
 template <class T>
-__device__ __forceinline__ F8 load8(const T* row, int col, int n, bool aligned) {
-  if (aligned && col + 8 <= n) return load8_whole(row + col);
+__device__ __forceinline__ F8 load8(const T* row, int col, int n) {
+  if (col + 8 <= n) return load8_whole(row + col);
   F8 v;
   v.lo = load4_edge(row, col, n);
   v.hi = load4_edge(row, col + 4, n);
   return v;
 }
 template <class T>
-__device__ __forceinline__ void store8(T* row, int col, int n, bool aligned, const F8& v) {
-  if (aligned && col + 8 <= n) {
+__device__ __forceinline__ void store8(T* row, int col, int n, const F8& v) {
+  if (col + 8 <= n) {
     store8_whole(row + col, v);
   } else {
     store4_edge(row, col, n, v.lo);

@@ -253,28 +253,6 @@ template <int BM, int BN, int WM, int WN>
 struct Turned {
   static constexpr int CR = WM < 64 ? WM : 64, PITCH = WN + 4, BYTES = CR * PITCH * 4;
 };
-// Eight columns of a row that allows 16-byte accesses: n is a multiple of 8, or of 4 in fp32, where the
-// last group may be half there.
-template <class T>
-__device__ __forceinline__ F8 load8_edge4(const T* row, int col, int n) {
-  if constexpr (sizeof(T) == 4) {
-    F8 v;
-    v.lo = *reinterpret_cast<const f4*>(row + col);
-    v.hi = col + 4 < n ? *reinterpret_cast<const f4*>(row + col + 4) : f4zero();
-    return v;
-  } else {
-    return load8_whole(row + col);
-  }
-}
-template <class T>
-__device__ __forceinline__ void store8_edge4(T* row, int col, int n, const F8& v) {
-  if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<f4*>(row + col) = v.lo;
-    if (col + 4 < n) *reinterpret_cast<f4*>(row + col + 4) = v.hi;
-  } else {
-    store8_whole(row + col, v);
-  }
-}
 // the wave's LDS accesses before are done before those after
 __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -448,8 +426,7 @@ __global__ __launch_bounds__(256, OCC) void k_dense(const GemmArgs a, const EpiD
     // The wave's sub-tile goes through its own part of LDS, CR rows at a time, so that a lane gets eight
     // columns of a row (one generator call, one 16-byte access) and neighbouring lanes the row's next
     // ones: rows of 16 lanes' accesses instead of pieces of 32 bytes, and a loop instead of a body for
-    // every accumulator.  U row groups at a time have their residual loads in flight together.  Rows
-    // that 16-byte accesses do not fit (an odd n) go back to LDS and out column by column.
+    // every accumulator.  U row groups at a time have their residual loads in flight together.
     typedef Turned<BM, BN, WM, WN> TU;
     constexpr int CR = TU::CR, PITCH = TU::PITCH, LPR = WN / 8, RPI = 64 / LPR, IT = CR / RPI;
     constexpr int U = BIG ? 4 : 2;
@@ -457,9 +434,8 @@ __global__ __launch_bounds__(256, OCC) void k_dense(const GemmArgs a, const EpiD
     float* const mine = reinterpret_cast<float*>(smem + wave * TU::BYTES);
     const uint64_t sub = e.drop.thr ? drop_sub(e.drop) : 0;
     const int lc = (lane % LPR) * 8, lr = lane / LPR, col = j0 + wj + lc;
-    const bool whole = e.vec_y && (!e.res || e.vec_r);  // n is a multiple of 8 (fp32: of 4) then
     F8 b{f4zero(), f4zero()};
-    if (e.bias && col < e.n) b = load8((const T*)e.bias, col, e.n, false);
+    if (e.bias && col < e.n) b = load8((const T*)e.bias, col, e.n);
     auto out = [&](auto chunk) __attribute__((always_inline)) {
       constexpr int CH = decltype(chunk)::value;
 #pragma unroll
@@ -468,53 +444,36 @@ __global__ __launch_bounds__(256, OCC) void k_dense(const GemmArgs a, const EpiD
         for (int j = 0; j < NI; ++j)
           *reinterpret_cast<f4*>(&mine[(16 * i + (lane & 15)) * PITCH + 16 * j + 4 * g]) = acc[CH * (CR / 16) + i][j];
       wave_sync();
-      const int row0 = i0 + wi + CH * CR;
-      if (col < e.n)
-        with_act(e.act, [&](auto act) __attribute__((always_inline)) {
-          constexpr int ACT = decltype(act)::value;
+      if (col < e.n) {
 #pragma unroll 1
-          for (int it = 0; it < IT; it += U) {
-            F8 res[U];
-            const int r = it * RPI + lr;
-            if (e.res && whole) {
+        for (int it = 0; it < IT; it += U) {
+          F8 res[U], v[U];
+          const int r = it * RPI + lr, row = i0 + wi + CH * CR + r;
 #pragma unroll
-              for (int u = 0; u < U; ++u)
-                if (row0 + r + u * RPI < a.I)
-                  res[u] = load8_edge4<T>((const T*)e.res + (int64_t)(row0 + r + u * RPI) * e.ldr, col, e.n);
-            }
+          for (int u = 0; u < U; ++u) {
+            if (e.res && row + u * RPI < a.I) res[u] = load8((const T*)e.res + (int64_t)(row + u * RPI) * e.ldr, col, e.n);
+            const float* p = &mine[(r + u * RPI) * PITCH + lc];
+            v[u].lo = *reinterpret_cast<const f4*>(p);
+            v[u].hi = *reinterpret_cast<const f4*>(p + 4);
+          }
+          with_act(e.act, [&](auto act) __attribute__((always_inline)) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-              const int row = row0 + r + u * RPI;
-              if (row >= a.I) continue;
-              float* p = &mine[(r + u * RPI) * PITCH + lc];
-              F8 v;
-              v.lo = *reinterpret_cast<const f4*>(p);
-              v.hi = *reinterpret_cast<const f4*>(p + 4);
-              v = value_of<T, ACT>(e, row, col, sub, v, b);
-              if (whole) {
-                if (e.res) {
-                  v.lo += res[u].lo;
-                  v.hi += res[u].hi;
-                }
-                store8_edge4<T>((T*)e.y + (int64_t)row * e.ldy, col, e.n, v);
-              } else {
-                *reinterpret_cast<f4*>(p) = v.lo;
-                *reinterpret_cast<f4*>(p + 4) = v.hi;
-              }
+            for (int u = 0; u < U; ++u)
+              if (row + u * RPI < a.I)
+                v[u] = value_of<T, decltype(act)::value>(e, row + u * RPI, col, sub, v[u], b);
+          });
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            if (row + u * RPI >= a.I) continue;
+            if (e.res) {
+              v[u].lo += res[u].lo;
+              v[u].hi += res[u].hi;
             }
+            store8((T*)e.y + (int64_t)(row + u * RPI) * e.ldy, col, e.n, v[u]);
           }
-        });
-      wave_sync();
-      if (!whole) {
-        const int width = min(WN, e.n - j0 - wj), rows = min(CR, a.I - row0);
-        for (int r = lane / WN; r < rows; r += 64 / WN > 0 ? 64 / WN : 1)
-          for (int c = lane % WN; c < width; c += 64) {
-            float v = mine[r * PITCH + c];
-            if (e.res) v += (float)((const T*)e.res)[(int64_t)(row0 + r) * e.ldr + j0 + wj + c];
-            ((T*)e.y)[(int64_t)(row0 + r) * e.ldy + j0 + wj + c] = (T)v;
-          }
-        wave_sync();
+        }
       }
+      wave_sync();
     };
     out(std::integral_constant<int, 0>());
     if constexpr (WM / CR == 2) out(std::integral_constant<int, 1>());
