@@ -32,7 +32,7 @@ __global__ __launch_bounds__(256) void k_pack(const PackDev a, const PackDev b) 
   const int per = p.per();
   const int64_t q = (int64_t)(first ? blockIdx.x : blockIdx.x - na) * 256 + threadIdx.x;
   if (q >= (int64_t)p.rows * per) return;
-  const int64_t row = q / per;
+  const int64_t row = row_of(q, per);
   const int col = (int)(q - row * per) * 8;
   const F8 v = load8((const T*)p.in + row * p.ld, col, p.cols);
   store8_whole((T*)p.out + row * (per * 8) + col, v);
@@ -50,7 +50,7 @@ __global__ __launch_bounds__(256) void k_join(const float* __restrict__ part, in
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t q = (int64_t)blockIdx.x * 64 + lane;
   const bool live = q < rows * e.groups;
-  const int64_t row = live ? q / e.groups : 0;
+  const int64_t row = live ? row_of(q, e.groups) : 0;
   const int col = live ? (int)(q - row * e.groups) * 8 : 0, n = e.n;
   const int64_t stride = rows * ldp;
   F8 v{f4zero(), f4zero()};
@@ -352,7 +352,7 @@ __global__ __launch_bounds__(256) void k_dropout(const T* __restrict__ x, int64_
     }
     store8_whole(y + 8 * q, v);
   } else {
-    const int64_t row = q / groups;
+    const int64_t row = row_of(q, groups);
     const int col = (int)(q - row * groups) * 8;
     F8 v = load8(x + row * ldx, col, n);
     if (d.thr) v = drop8(v, drop_words(d, sub, (uint64_t)q), d);
@@ -620,8 +620,8 @@ hipError_t backward(const dgprf_linear_grad_t& a, Scratch& sc, hipStream_t st, b
     d.act = a.act;
     d.drop = drop_dev(a.drop_thr, a.seed, a.sub, a.step);
     const int64_t strips = cdiv(d.groups, 64);
-    // enough workgroups to fill the memory system, and 16 rows (four a wave) in each where there are many
-    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(cdiv(1024, strips), cdiv(m, 16)));
+    // workgroups enough to fill the chip, down to a row for each wave
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(cdiv(1024, strips), cdiv(m, 4)));
     d.rows_part = (int)up(cdiv(m, want), 4);
     const int64_t parts = cdiv(m, d.rows_part);
     if (a.db) d.part = (float*)sc.take(parts * d.ldz * 4);

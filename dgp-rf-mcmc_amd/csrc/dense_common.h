@@ -31,14 +31,21 @@ struct Vec {
 inline int elem_size(int dtype) { return dtype == DGPRF_F32 ? 4 : 2; }
 
 // ---------------------------------------------------------------- activations
-// Normal distribution function by its tail: for a = |z|, P(Z < -a) = e^{-a^2 / 2} Q(a) with
-// Q(a) = erfcx(a / sqrt 2) / 2, a smooth, slowly falling function fitted (least squares, reweighted
-// towards the smallest maximal relative error, a in [0, 14]) as t (c0 + c1 t + ...), t = 1 / (1 + ca).
-// The negative side keeps its relative precision (no 1 - erf cancellation) and the exponential is
-// the one the slope needs.  Degree 8: 3.2e-8 (4e-7 as evaluated in 32 bits); degree 5, for the
-// 16-bit types whose rounding is 2^-9 and more: 8.2e-6.
+// Normal distribution function by its tail P(Z < -a), a = |z|: the negative side keeps its relative
+// precision (no 1 - erf cancellation).  Both forms are own least-squares fits, reweighted towards the
+// smallest maximal relative error.
+//  * fp32: e^{-a^2 / 2} Q(a), Q(a) = erfcx(a / sqrt 2) / 2 = t (c0 + c1 t + ... + c8 t^8), t = 1 / (1 + 0.35 a),
+//    a in [0, 14]: 3.2e-8 (4e-7 as evaluated in 32 bits).
+//  * 16-bit types (whose rounding is 2^-12 and more): 2^{p(a)}, p of degree 7 fitted to log2 of the tail
+//    for a in [0, 6.5]: 8.3e-6 as evaluated, falling to 0 beyond; two instructions in three of the other.
+__device__ __forceinline__ float exp_of(float x) {  // e^x: v_exp_f32 is 2^x to 1 ulp
+  return __builtin_amdgcn_exp2f(x * 1.4426950408889634f);
+}
+__device__ __forceinline__ float gauss(float z) {  // e^{-z^2 / 2}
+  return __builtin_amdgcn_exp2f(z * z * -0.7213475204444817f);
+}
 template <class T>
-__device__ __forceinline__ float tail_q(float a) {
+__device__ __forceinline__ float tail_of(float a) {
   if constexpr (sizeof(T) == 4) {
     const float t = __builtin_amdgcn_rcpf(fmaf(0.35f, a, 1.f));
     float p = -0.02914646826684475f;
@@ -50,24 +57,17 @@ __device__ __forceinline__ float tail_q(float a) {
     p = fmaf(p, t, 0.11983250081539154f);
     p = fmaf(p, t, 0.13986191153526306f);
     p = fmaf(p, t, 0.13962140679359436f);
-    return p * t;
+    return p * t * gauss(a);
   } else {
-    const float t = __builtin_amdgcn_rcpf(fmaf(0.3f, a, 1.f));
-    float p = -0.07709866762161255f;
-    p = fmaf(p, t, 0.21604043245315552f);
-    p = fmaf(p, t, -0.016951488330960274f);
-    p = fmaf(p, t, 0.1441979855298996f);
-    p = fmaf(p, t, 0.11374157667160034f);
-    p = fmaf(p, t, 0.12007425725460052f);
-    return p * t;
+    float p = -1.7577908693056088e-06f;
+    p = fmaf(p, a, 5.993694139760919e-05f);
+    p = fmaf(p, a, -0.0009163665818050504f);
+    p = fmaf(p, a, 0.008447404019534588f);
+    p = fmaf(p, a, -0.05382455512881279f);
+    p = fmaf(p, a, -0.45861563086509705f);
+    p = fmaf(p, a, -1.1511802673339844f);
+    return __builtin_amdgcn_exp2f(fmaf(p, a, -1.0000038146972656f));
   }
-}
-
-__device__ __forceinline__ float exp_of(float x) {  // e^x: v_exp_f32 is 2^x to 1 ulp
-  return __builtin_amdgcn_exp2f(x * 1.4426950408889634f);
-}
-__device__ __forceinline__ float gauss(float z) {  // e^{-z^2 / 2}
-  return __builtin_amdgcn_exp2f(z * z * -0.7213475204444817f);
 }
 __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + exp_of(-z)); }
 // sqrt(2 / pi) (z + 0.044715 z^3), twice: tanh u = 2 sigmoid(2 u) - 1, so 0.5 z (1 + tanh u) = z sigmoid(2 u)
@@ -79,7 +79,7 @@ template <class T, int ACT>
 __device__ __forceinline__ float act_of(float z) {
   if constexpr (ACT == DGPRF_ACT_RELU) return z < 0.f ? 0.f : z;  // a NaN stays one
   if constexpr (ACT == DGPRF_ACT_GELU) {
-    const float tail = tail_q<T>(fabsf(z)) * gauss(z);
+    const float tail = tail_of<T>(fabsf(z));
     return z * (z < 0.f ? tail : 1.f - tail);
   }
   if constexpr (ACT == DGPRF_ACT_GELU_TANH) return z * sigmoid(tanh_arg2(z));
@@ -94,8 +94,8 @@ __device__ __forceinline__ float slope_of(float z) {
   const float zc = __builtin_amdgcn_fmed3f(z, -60.f, 60.f);
   if constexpr (ACT == DGPRF_ACT_RELU) return z > 0.f ? 1.f : 0.f;
   if constexpr (ACT == DGPRF_ACT_GELU) {
-    const float e = gauss(z), tail = tail_q<T>(fabsf(z)) * e;
-    return fmaf(zc * 0.3989422804014327f, e, z < 0.f ? tail : 1.f - tail);
+    const float tail = tail_of<T>(fabsf(z));
+    return fmaf(zc * 0.3989422804014327f, gauss(z), z < 0.f ? tail : 1.f - tail);
   }
   if constexpr (ACT == DGPRF_ACT_GELU_TANH) {
     // g = sigmoid(2u): g + z g (1 - g) 2u'
@@ -146,13 +146,31 @@ struct DropDev {
 __device__ __forceinline__ uint64_t drop_sub(const DropDev& d) {
   return d.sub + (d.step ? (uint64_t)*d.step : 0ull);
 }
+// philox4x32_10 of dgprf_device.h with the three-input exclusive or of gfx950: a fifth fewer instructions
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96);
+#else
+  return a ^ b ^ c;
+#endif
+}
+__device__ __forceinline__ u32x4 philox_words(u32x4 c, uint32_t k0, uint32_t k1) {
+#pragma unroll
+  for (int i = 0; i < 10; ++i) {
+    const uint64_t p0 = (uint64_t)0xD2511F53u * c.x, p1 = (uint64_t)0xCD9E8D57u * c.z;
+    c = u32x4{xor3((uint32_t)(p1 >> 32), c.y, k0), (uint32_t)p1, xor3((uint32_t)(p0 >> 32), c.w, k1), (uint32_t)p0};
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  return c;
+}
 __device__ __forceinline__ u32x4 drop_words(const DropDev& d, uint64_t sub, uint64_t q) {
   u32x4 c;
   c.x = (uint32_t)q;
   c.y = (uint32_t)sub;
   c.z = (uint32_t)(sub >> 32);
   c.w = ((uint32_t)DGPRF_RNG_DROPOUT << 24) | ((uint32_t)(q >> 32) & 0x00FFFFFFu);
-  return philox4x32_10(c, d.k0, d.k1);
+  return philox_words(c, d.k0, d.k1);
 }
 // keep or drop elements 2 i and 2 i + 1 by word i
 __device__ __forceinline__ float drop_lo(float v, uint32_t word, const DropDev& d) {
@@ -191,6 +209,10 @@ __device__ __forceinline__ void store4_edge(T* row, int col, int n, f4 v) {
 }
 
 // ---------------------------------------------------------------- eight columns of a row
+// row and group of the q-th of rows x groups (a 64-bit division takes some hundred instructions)
+__device__ __forceinline__ int64_t row_of(int64_t q, int groups) {
+  return q >> 32 ? q / groups : (int64_t)((uint32_t)q / (uint32_t)groups);
+}
 struct F8 {
   f4 lo, hi;
 };
