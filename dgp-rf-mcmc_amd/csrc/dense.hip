@@ -398,7 +398,7 @@ Shape shape_of(int64_t I, int64_t J, int64_t K, int es) {
     const int64_t mt = cdiv(I, ts.bm), nt = cdiv(J, ts.bn), stages = cdiv(K * es, ts.kb);
     if (mt * nt >= (int64_t)1 << 26) continue;  // workgroups of a launch, times 32 parts at most
     for (int64_t want = 1; want <= 32; want *= 2) {
-      if (want > 1 && stages < 4 * want) break;
+      if (want > 1 && (stages < 4 * want || mt * nt > 1024)) break;
       const int64_t per = cdiv(stages, want), parts = cdiv(stages, per);
       const float k = (float)per * ts.kb / es / 1024.f, rounds = (float)cdiv(mt * nt * parts, 256);
       float t = tc.fixed + rounds * (tc.out + tc.rate * k);
@@ -546,8 +546,11 @@ int check_dims(int32_t dtype, int32_t act, int64_t m, int64_t k, int64_t n, int6
   if (m < 0 || k < 1 || n < 1 || ldx < k || ldw < n) return DGPRF_E_SHAPE;
   if (m >= ((int64_t)1 << 31) || k > kMaxWidth || n > kMaxWidth || ldx > kMaxWidth || ldw > kMaxWidth)
     return DGPRF_E_SHAPE;
-  // workgroups of the per-eight-columns kernels
-  if (m * cdiv(std::max(k, n), 8) >= ((int64_t)1 << 39)) return DGPRF_E_SHAPE;
+  // workgroups of a launch: of 256 groups of eight columns, and of 128 x 128 tiles
+  const int64_t w = std::max(k, n);
+  if (m * cdiv(w, 8) >= ((int64_t)1 << 39) || cdiv(m, 128) * cdiv(w, 128) >= ((int64_t)1 << 26) ||
+      cdiv(k, 128) * cdiv(n, 128) >= ((int64_t)1 << 26))
+    return DGPRF_E_SHAPE;
   return DGPRF_OK;
 }
 
@@ -600,7 +603,8 @@ hipError_t backward(const dgprf_linear_grad_t& a, Scratch& sc, hipStream_t st, b
   hipError_t err = hipSuccess;
   // dz, unless it is dy and dy can be read in place
   const bool products = a.dx || a.dw;
-  const bool same = a.act == DGPRF_ACT_NONE && a.drop_thr == 0 && in_place(a.dy, a.lddy, n, es);
+  // (rows that share memory are copied apart: their product's K range has no end to check against)
+  const bool same = a.act == DGPRF_ACT_NONE && a.drop_thr == 0 && a.lddy >= n && in_place(a.dy, a.lddy, n, es);
   const void* dz = a.dy;
   int64_t lddz = a.lddy, na = n;
   if (products && !same) {

@@ -1,0 +1,73 @@
+"""DenseLayer and DropoutLayer: layers trained by gradient, for the networks around the random-feature
+layers — a feature extractor below a DGP, the deterministic or MC-dropout network beside it.
+
+They call dgprf.linear / dgprf.dropout (one kernel for product, bias, activation, dropout and residual)
+and are differentiable: torch.autograd.grad(loss, layer.trainable_variables) and
+experiments.optimizers.Adam.apply_gradients train them.  The product is GPLayer's (X W, W [in, out]).
+"""
+import torch
+
+from dgprf import _native as N
+from dgprf import engine as E
+from dgprf.dense import dropout, linear
+from dgprf.module import Module
+
+
+def _input(X, n, dtype):
+    """X [..., n] on the device in the layer's type (a tensor that is, is taken as it is)."""
+    if not torch.is_tensor(X):
+        X = torch.as_tensor(X)
+    if X.dim() < 1 or X.shape[-1] != n:
+        raise ValueError(f"X must be [..., {n}], got {tuple(X.shape)}")
+    return X.to(device=E.device(), dtype=dtype)
+
+
+class DenseLayer(Module):
+    """residual + D(a(X W + b)): W ~ N(0, 1 / in_feature), b = 0.
+
+    activation: none, relu, gelu, gelu_tanh or silu; dropout: the probability of an element's being
+    dropped, while set_training(True) holds; dtype: float32, float16 or bfloat16."""
+
+    def __init__(self, in_feature, out_feature, activation="none", bias=True, dropout=0.,
+                 dtype=torch.float32, name=None):
+        super().__init__(name=name)
+        if activation not in N.ACTS:
+            raise ValueError(f"activation must be one of {', '.join(N.ACTS)}, got {activation!r}")
+        if not 0. <= dropout <= 1.:
+            raise ValueError(f"dropout probability must be in [0, 1], got {dropout}")
+        self.in_feature, self.out_feature = int(in_feature), int(out_feature)
+        self.activation, self.dropout, self.training = activation, float(dropout), False
+        w = E.normal((self.in_feature, self.out_feature), N.RNG_W) * self.in_feature ** -0.5
+        self.W = w.to(dtype).requires_grad_()
+        self.W.trainable, self.W.var_name = True, "dense_layer_W"
+        self.b = None
+        if bias:
+            self.b = torch.zeros(self.out_feature, dtype=dtype, device=w.device, requires_grad=True)
+            self.b.trainable, self.b.var_name = True, "dense_layer_b"
+
+    def __call__(self, X, residual=None, seed=None, sub=None, step=None):
+        """X [..., in_feature] -> [..., out_feature]; seed, sub, step: the mask's, as in dgprf.linear."""
+        X = _input(X, self.in_feature, self.W.dtype)
+        return linear(X, self.W, self.b, self.activation, residual,
+                      self.dropout if self.training else 0., seed, sub, step)
+
+    def set_training(self, state):
+        self.training = bool(state)
+
+
+class DropoutLayer(Module):
+    """residual + D(X), while set_training(True) holds; X as it is (plus the residual) otherwise."""
+
+    def __init__(self, p, name=None):
+        super().__init__(name=name)
+        if not 0. <= p <= 1.:
+            raise ValueError(f"dropout probability must be in [0, 1], got {p}")
+        self.p, self.training = float(p), False
+
+    def __call__(self, X, residual=None, seed=None, sub=None, step=None):
+        if self.training:
+            return dropout(X, self.p, residual, seed, sub, step)
+        return X if residual is None else X + residual
+
+    def set_training(self, state):
+        self.training = bool(state)

@@ -69,15 +69,18 @@ def test_calls_refused_before_anything_is_enqueued():
     assert lib.dgprf_linear_scratch(e(linear()), None) == N.E_ARG
     assert lib.dgprf_linear_forward(e(linear()), None, 0, None) == N.E_ARG      # no tensors
     some = 1 << 20  # never read: refused on the host
-    ok = dict(x=some, w=some, y=some)
-    assert scratch(linear(**ok))[1] > 0
+    ok = dict(x=some, w=some, y=some, m=1, k=1 << 14, ldx=1 << 14)  # one row of a long K: parts to join
+    assert scratch(linear(**ok)) == (0, scratch(linear(**ok))[1]) and scratch(linear(**ok))[1] > 1
     assert lib.dgprf_linear_forward(e(linear(**ok)), None, 0, None) == N.E_ARG   # scratch missing
     assert lib.dgprf_linear_forward(e(linear(**ok)), some, 1, None) == N.E_ARG   # scratch too small
     assert lib.dgprf_linear_forward(e(linear(res=some, ldr=3, **ok)), some, 1 << 30, None) == N.E_SHAPE
     assert lib.dgprf_linear_forward(e(linear(act=2, aux=some + 4, **ok)), some, 1 << 30, None) == N.E_ARG
-    g = dict(x=some, w=some, dy=some, dx=some)
+    g = dict(x=some, w=some, dy=some, dx=some, drop_thr=1)  # dz is a tensor of its own
+    assert scratch(grad(**g))[1] > 1
     assert lib.dgprf_linear_backward(e(grad(act=2, **g)), some, 1 << 30, None) == N.E_ARG  # nothing saved
     assert lib.dgprf_linear_backward(e(grad(lddy=3, **g)), some, 1 << 30, None) == N.E_SHAPE
+    assert lib.dgprf_linear_backward(e(grad(**g)), None, 0, None) == N.E_ARG
+    assert lib.dgprf_linear_backward(e(grad(**{**g, "w": None})), some, 1 << 30, None) == N.E_ARG
     assert lib.dgprf_dropout(9, some, 1, 8, 8, None, 0, 0, 0, 0, None, some, None) == N.E_ARG
     assert lib.dgprf_dropout(0, some, 1, 8, 8, None, 0, 65537, 0, 0, None, some, None) == N.E_ARG
     assert lib.dgprf_dropout(0, some, 2, 8, 4, None, 0, 1, 0, 0, None, some, None) == N.E_SHAPE
@@ -104,3 +107,18 @@ def test_python_refusals():
         with pytest.raises(ValueError):
             dgprf.dense.drop_threshold(p)
     assert [dgprf.dense.drop_threshold(p) for p in (0, 0.1, 0.5, 1)] == [0, 6554, 32768, 65536]
+
+
+def test_layer_refusals():
+    from layers import DenseLayer, DropoutLayer
+    for bad in (lambda: DenseLayer(4, 8, activation="tanh"), lambda: DenseLayer(4, 8, dropout=2.0),
+                lambda: DropoutLayer(-0.5)):
+        with pytest.raises(ValueError):
+            bad()
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="checks the no-GPU refusal")
+def test_layer_needs_a_device():
+    from layers import DenseLayer
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        DenseLayer(4, 8)

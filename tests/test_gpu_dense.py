@@ -400,3 +400,126 @@ def test_rows_around_are_left_alone():
            ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
     torch.cuda.synchronize()
     assert bool((y[:m] == k).all()) and bool((y[m:] == 7).all())
+
+
+def test_gradients_that_share_rows():
+    """The gradient of a sum over rows is one row for all: its products and sums, an infinite element
+    among them where the products have no other."""
+    g = _gen(9)
+    for m, act, p in ((5, "none", 0.0), (70, "none", 0.0), (200, "gelu", 0.3)):
+        x, w, b = (grid(g, *s).to(DEV).requires_grad_() for s in ((m, 40), (40, 56), (56,)))
+        y = dgprf.linear(x, w, b, act, dropout=p, seed=1, sub=2)
+        row = grid(g, 1, 56).to(DEV)
+        got = torch.autograd.grad(y, (x, w, b), row.expand(m, 56), retain_graph=True)
+        want = torch.autograd.grad(y, (x, w, b), row.expand(m, 56).contiguous(), retain_graph=True)
+        assert all(torch.equal(u, v) for u, v in zip(got, want))
+        one = torch.autograd.grad(y.sum(), (x, w, b), retain_graph=True)
+        want = torch.autograd.grad(y, (x, w, b), torch.ones_like(y))
+        assert all(torch.equal(u, v) for u, v in zip(one, want))
+    x = torch.ones(70, 40, device=DEV)
+    w = torch.ones(40, 56, device=DEV, requires_grad=True)
+    row = torch.ones(1, 56, device=DEV)
+    row[0, 3] = float("inf")
+    dw, = torch.autograd.grad(dgprf.linear(x, w), w, row.expand(70, 56))
+    assert bool(torch.isinf(dw[:, 3]).all()) and bool((dw[:, :3] == 70).all()) and bool((dw[:, 4:] == 70).all())
+
+
+def test_refusals():
+    x, w = torch.zeros(4, 8, device=DEV), torch.zeros(8, 16, device=DEV)
+    for bad in (lambda: dgprf.linear(x, w.half()), lambda: dgprf.linear(x.double(), w.double()),
+                lambda: dgprf.linear(x, w, torch.zeros(16, device=DEV).bfloat16()),
+                lambda: dgprf.linear(x, w, residual=torch.zeros(4, 16, device=DEV).half()),
+                lambda: dgprf.dropout(x, 0.5, residual=x.half()), lambda: dgprf.dropout(x.long(), 0.5)):
+        with pytest.raises(TypeError):
+            bad()
+    for bad in (lambda: dgprf.linear(x, w[:7]), lambda: dgprf.linear(x, w[0]), lambda: dgprf.linear(x, w, x[0]),
+                lambda: dgprf.linear(x, w, residual=x), lambda: dgprf.linear(x, w[:, :0]),
+                lambda: dgprf.linear(x[:, :0], w[:0]), lambda: dgprf.linear(x, w.cpu()),
+                lambda: dgprf.linear(x, w, activation="tanh"), lambda: dgprf.linear(x, w, dropout=1.5),
+                lambda: dgprf.linear(x, w, residual=torch.zeros(1, 16, device=DEV)),
+                lambda: dgprf.linear(x, w, dropout=0.5, step=torch.zeros(1, device=DEV)),
+                lambda: dgprf.linear(x, w, dropout=0.5, step=torch.zeros(1, dtype=torch.int64)),
+                lambda: dgprf.dropout(x, -0.1), lambda: dgprf.dropout(x, 0.5, residual=x[:2]),
+                lambda: dgprf.linear(torch.zeros(2, (1 << 20) + 8, device=DEV)[:, :8].as_strided((2, 8), ((1 << 20) + 8, 1)), w)):
+        with pytest.raises(ValueError):
+            bad()
+    # what backward needs was changed in between
+    wg = w.clone().requires_grad_()
+    step = torch.zeros(1, dtype=torch.int64, device=DEV)
+    y = dgprf.linear(x, wg, dropout=0.5, seed=1, sub=1, step=step)
+    step += 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y.sum(), wg)
+
+
+def test_offsets_past_32_bits():
+    """65,600 rows of 32,768 elements: the last rows of a result, and gradients over all of them."""
+    m, k, n, t = 65600, 16, 32768, torch.bfloat16
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB")
+    g = torch.Generator(device=DEV)
+    g.manual_seed(1)
+    x = torch.randint(-2, 3, (m, k), generator=g, device=DEV).to(t).requires_grad_()
+    w = torch.randint(-2, 3, (k, n), generator=g, device=DEV).to(t).requires_grad_()
+    y = dgprf.linear(x, w, dropout=0.5, seed=3, sub=4)
+    tail = slice(m - 300, m)
+    part = keep_rows(m - 300, 300, n, 32768, 3, 4).to(DEV)
+    want = torch.where(part, 2 * (x[tail].float() @ w.float()), torch.zeros((), device=DEV)).to(t)
+    assert torch.equal(y[tail], want)
+    assert torch.equal(dgprf.dropout(torch.ones_like(y), 0.5, seed=3, sub=4)[tail] != 0, part)
+    # a gradient of the tail alone, so that the sums are exact
+    dy = torch.zeros_like(y)
+    dy[tail] = 1
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    dz = 2 * part.float()
+    assert not bool(dx[: m - 300].any()) and torch.equal(dx[tail], (dz @ w.float().t().contiguous()).to(t))
+    assert torch.equal(dw, (x[tail].float().t().contiguous() @ dz).to(t))
+
+
+def keep_rows(first, rows, n, thr, seed, sub):
+    """keep_mask's rows first .. first + rows - 1 (groups numbered from row 0)."""
+    from oracle import rng
+    groups = -(-n // 8)
+    ctr = np.zeros((rows * groups, 4), dtype=np.uint64)
+    q = np.arange(first * groups, (first + rows) * groups, dtype=np.uint64)
+    ctr[:, 0], ctr[:, 1], ctr[:, 2] = q & np.uint64(0xFFFFFFFF), sub & 0xFFFFFFFF, sub >> 32
+    ctr[:, 3] = (q >> np.uint64(32)) + np.uint64(8 << 24)
+    h = np.ascontiguousarray(rng.philox4x32_10(ctr, (seed & 0xFFFFFFFF, seed >> 32))).view(np.uint16)
+    return torch.from_numpy(np.ascontiguousarray(h.reshape(rows, groups * 8)[:, :n] >= thr))
+
+
+def test_layers():
+    """DenseLayer / DropoutLayer: the functions' results and gradients, inside a stack with the
+    random-feature layers, and an optimizer's step by its formula."""
+    from experiments.optimizers import Adam
+    from kernels import RBFKernel
+    from layers import DenseLayer, DropoutLayer, GPLayer, RBFLayer
+    from utils import BNN_from_list
+    dgprf.set_seed(5)
+    up, down, drop = DenseLayer(6, 40, "silu", dropout=0.2), DenseLayer(40, 6, bias=False), DropoutLayer(0.5)
+    assert [tuple(v.shape) for v in up.trainable_variables] == [(6, 40), (40,)]
+    assert len(down.trainable_variables) == 1 and drop.trainable_variables == ()
+    X = np.random.default_rng(0).standard_normal((50, 6))
+    x = torch.as_tensor(X, dtype=torch.float32).to(DEV)
+    assert torch.equal(up(X), dgprf.linear(x, up.W, up.b, "silu")) and drop(x) is x
+    up.set_training(True)
+    drop.set_training(True)
+    h = up(X, seed=1, sub=2)
+    assert torch.equal(h, dgprf.linear(x, up.W, up.b, "silu", dropout=0.2, seed=1, sub=2))
+    y = drop(down(h, residual=x), seed=1, sub=3)
+    variables = up.trainable_variables + down.trainable_variables
+    grads = torch.autograd.grad(y.square().sum(), variables)
+    y2 = dgprf.dropout(dgprf.linear(h.detach(), down.W, residual=x), 0.5, seed=1, sub=3)
+    dw, = torch.autograd.grad(y2.square().sum(), down.W)
+    assert torch.equal(grads[2], dw)
+    before = [v.detach().clone() for v in variables]
+    Adam(learning_rate=0.01).apply_gradients(zip(grads, variables))
+    for v, b, gr in zip(variables, before, grads):  # the first step: m / sqrt(v) is the gradient's sign
+        assert torch.allclose(v.detach(), b - 0.01 * gr / (gr.abs() + 1e-7 / 0.001 ** 0.5), rtol=1e-5, atol=2e-7)
+    net = BNN_from_list([DenseLayer(6, 16, "gelu"), DenseLayer(16, 3), RBFLayer(RBFKernel(3, is_ard=True), 20),
+                         GPLayer(40, 2)])
+    assert net(X).shape == (50, 2) and bool(torch.isfinite(net(X)).all())
+    half = DenseLayer(6, 8, dtype=torch.bfloat16)
+    assert half(X).dtype == torch.bfloat16
+    with pytest.raises(ValueError):
+        half(X[:, :5])
