@@ -53,8 +53,12 @@ __global__ __launch_bounds__(256) void k_join(const float* __restrict__ part, in
   const int64_t row = live ? row_of(q, e.groups) : 0;
   const int col = live ? (int)(q - row * e.groups) * 8 : 0, n = e.n;
   const int64_t stride = rows * ldp;
-  F8 v{f4zero(), f4zero()};
+  F8 v{f4zero(), f4zero()}, b{f4zero(), f4zero()}, r{f4zero(), f4zero()};
   if (live) {
+    if (wave == 0) {  // on their way with the parts
+      if (e.bias) b = load8((const T*)e.bias, col, n);
+      if (e.res) r = load8((const T*)e.res + row * e.ldr, col, n);
+    }
     const float* p = part + row * ldp + col;  // ldp % 8 == 0
 #pragma unroll 4
     for (int s = wave; s < parts; s += 4) {
@@ -73,12 +77,9 @@ __global__ __launch_bounds__(256) void k_join(const float* __restrict__ part, in
     v.lo += sums[w][0][lane];
     v.hi += sums[w][1][lane];
   }
-  F8 b{f4zero(), f4zero()};
-  if (e.bias) b = load8((const T*)e.bias, col, n);
   const uint64_t sub = e.drop.thr ? drop_sub(e.drop) : 0;
   with_act(e.act, [&](auto act) { v = value_of<T, decltype(act)::value>(e, row, col, sub, v, b); });
   if (e.res) {
-    const F8 r = load8((const T*)e.res + row * e.ldr, col, n);
     v.lo += r.lo;
     v.hi += r.hi;
   }
@@ -194,6 +195,11 @@ __global__ __launch_bounds__(1024) void k_strip(const T* __restrict__ x, const T
     const int k = kl + u * KL;
     v[u] = k < K && col < e.n ? load_piece<T>(w + (int64_t)k * ldw + col, e.n - col) : (vec)(T)0.f;
   }
+  const int c0 = strip * STRIP + tid * 8;
+  const bool out = tid < STRIP / 8 && c0 < e.n;  // this thread has eight columns of the result
+  F8 z{f4zero(), f4zero()}, b{f4zero(), f4zero()}, r{f4zero(), f4zero()};
+  if (out && e.bias) b = load8((const T*)e.bias, c0, e.n);
+  if (out && e.res) r = load8((const T*)e.res, c0, e.n);
   for (int k = tid; k < K; k += 1024) xs[k] = (float)x[k];
   __syncthreads();
   float acc[CE];
@@ -215,20 +221,16 @@ __global__ __launch_bounds__(1024) void k_strip(const T* __restrict__ x, const T
     if (lane < LPR) part[wave][lane * CE + c] = s;
   }
   __syncthreads();
-  const int c0 = strip * STRIP + tid * 8;
-  if (tid >= STRIP / 8 || c0 >= e.n) return;
-  F8 z{f4zero(), f4zero()}, b{f4zero(), f4zero()};
+  if (!out) return;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const f4* p = reinterpret_cast<const f4*>(&part[i][tid * 8]);
     z.lo += p[0];
     z.hi += p[1];
   }
-  if (e.bias) b = load8((const T*)e.bias, c0, e.n);
   const uint64_t sub = e.drop.thr ? drop_sub(e.drop) : 0;
   with_act(e.act, [&](auto act) { z = value_of<T, decltype(act)::value>(e, 0, c0, sub, z, b); });
   if (e.res) {
-    const F8 r = load8((const T*)e.res, c0, e.n);
     z.lo += r.lo;
     z.hi += r.hi;
   }
