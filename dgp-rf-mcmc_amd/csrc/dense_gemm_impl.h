@@ -5,9 +5,8 @@
 // A workgroup of four waves computes a BM x BN tile; a stage is KB bytes of K (64 or 128; 64 bytes
 // are 32 16-bit or 16 fp32 elements, one step of the matrix instructions).  Both operands' stages go
 // from memory to LDS without passing registers (16-byte buffer loads with the LDS destination) into
-// ST buffers, one barrier per stage.  The LDS
-// image of a load is linear in the lane, so bank conflicts are avoided by permuting which 16 bytes of
-// the source each lane fetches (XOR on the 16-byte index).
+// ST buffers, one barrier per stage.  The LDS image of a load is linear in the lane, so bank conflicts
+// are avoided by permuting which 16 bytes of the source each lane fetches (XOR on the 16-byte index).
 //  * K-contiguous operand: rows of KB bytes, the slots permuted so that eight neighbouring rows' equal
 //    chunks fall on all banks; a lane's MFMA fragment is one ds_read_b128.
 //  * K-strided operand: rows of one k.  16-bit fragments come from two ds_read_b64_tr_b16 (a 16-lane
@@ -17,6 +16,19 @@
 //
 // Edges: rows / columns past I, J fetch the last row again or zeros, and are not stored; K past the
 // end fetches zeros (offsets past the buffer descriptor's range read 0 without an access).
+//
+// Tiles (launch_layout), and what bounds them:
+//  * 256 x 256, 16-bit: a wave's 128 x 128 sub-tile takes a register file of accumulators and the fewest
+//    bytes from LDS (reads and the loads' writes 75 % of the matrix instructions' time; 128 x 64 a wave
+//    would be at 112 %).  One workgroup a CU, 128-byte rows of K (whole cache lines: 4096^3 in bf16 97 us,
+//    103 with 64-byte rows).  4096 x 8192 x 4096 in bf16: 183 us, 1.5 PFLOP/s, where a large library
+//    product of the type reaches 1.26; bound by the matrix instructions at the clock that they allow.
+//  * 256 x 128 (16-bit) and 128 x 128: two workgroups a CU, one's epilogue beside the other's product;
+//    bound by LDS.
+//  * 64 x 64: for results of few tiles.  fp32 takes two groups of four waves, one for each step of a
+//    stage, whose sums are added at the end (1024 x 2048 x 1024: 40 us, 43 with one); 16-bit steps are
+//    too short for that (1024 x 2048 x 2048 in bf16: 19 us, 16 with one).
+//  * 32 x 128: for few rows; bound by the memory's rate (24 x 8192 x 2048 in fp16: 6.8 us, 4.9 TB/s).
 #pragma once
 
 #include <algorithm>
@@ -152,21 +164,22 @@ struct Frags {
   typedef typename std::conditional<sizeof(T) == 4, f4, typename Vec<T>::v8>::type frag;
   static constexpr int KS = KB / 64;  // steps of a stage
   uint32_t at[KC ? KS : NF];
-  __device__ __forceinline__ void init(int w0, int lane) {
+  // ks0: the step that read() calls 0
+  __device__ __forceinline__ void init(int w0, int lane, int ks0) {
     const int g = lane >> 4, i = lane & 15;
     if constexpr (KC) {
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) at[ks] = (w0 + i) * KB + (((ks * 4 + g) ^ swz_row<KB>(i)) * 16);
+      for (int ks = 0; ks < KS; ++ks) at[ks] = (w0 + i) * KB + ((((ks + ks0) * 4 + g) ^ swz_row<KB>(i)) * 16);
     } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
       for (int f = 0; f < NF; ++f) {
-        const int c = (w0 + 16 * f) / 4, k = 4 * g;
+        const int c = (w0 + 16 * f) / 4, k = 16 * ks0 + 4 * g;
         at[f] = k * R * 4 + ((c + (i >> 2)) ^ swz_strided<T, R>(k)) * 16 + (i & 3) * 4;
       }
     } else {
 #pragma unroll
       for (int f = 0; f < NF; ++f) {
-        const int c = (w0 + 16 * f) / 8, k = 8 * g + (i >> 2);
+        const int c = (w0 + 16 * f) / 8, k = 32 * ks0 + 8 * g + (i >> 2);
         at[f] = k * R * 2 + ((c + ((i & 3) >> 1)) ^ swz_strided<T, R>(k)) * 16 + (i & 1) * 8;
       }
     }
@@ -252,6 +265,7 @@ __device__ __forceinline__ void settle(f4 (&acc)[MI][NI]) {
 template <int BM, int BN, int WM, int WN>
 struct Turned {
   static constexpr int CR = WM < 64 ? WM : 64, PITCH = WN + 4, BYTES = CR * PITCH * 4;
+  __device__ static int at(int wave, int from) { return from + wave * BYTES; }  // `from`: sums of the second group
 };
 // the wave's LDS accesses before are done before those after
 __device__ __forceinline__ void wave_sync() {
@@ -266,11 +280,12 @@ __device__ __forceinline__ void wait_loads() {
   __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | ((N >> 4) << 14));
 }
 
-template <class T, bool AKC, bool BKC, int BM, int BN, int WM, int WN, int KB, int ST, int OCC, bool PART>
-__global__ __launch_bounds__(256, OCC) void k_dense(const GemmArgs a, const EpiDev e) {
+template <class T, bool AKC, bool BKC, int BM, int BN, int WM, int WN, int KB, int ST, int OCC, int KG, bool PART>
+__global__ __launch_bounds__(256 * KG, OCC) void k_dense(const GemmArgs a, const EpiDev e) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host pass needs the stub alone
-  constexpr int NT = 256, MI = WM / 16, NI = WN / 16;
+  constexpr int NT = 256 * KG, MI = WM / 16, NI = WN / 16;
   static_assert(BM / WM * (BN / WN) == 4, "four waves");
+  static_assert(KG == 1 || KG == KB / 64, "a group of waves for each step of a stage");
   constexpr bool BIG = MI * NI == 64;  // accumulators fill a register file
   static_assert(!BIG || (MI == 8 && NI == 8 && sizeof(T) == 2 && BM == 256), "turn()'s groups");
   typedef Stage<T, AKC, BM, KB, NT> SA;
@@ -296,8 +311,8 @@ __global__ __launch_bounds__(256, OCC) void k_dense(const GemmArgs a, const EpiD
   }
   const int i0 = mt * BM, j0 = nt * BN;
   const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wi = wave / (BN / WN) * WM, wj = wave % (BN / WN) * WN;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wpos = wave % 4, group = wave / 4;
+  const int wi = wpos / (BN / WN) * WM, wj = wpos % (BN / WN) * WN;
 
   SA sa;
   SB sb;
@@ -310,8 +325,8 @@ __global__ __launch_bounds__(256, OCC) void k_dense(const GemmArgs a, const EpiD
   if (!PART && e.bias && col < e.n) b = load8((const T*)e.bias, col, e.n);
   FA fa;
   FB fb;
-  fa.init(wi, lane);
-  fb.init(wj, lane);
+  fa.init(wi, lane, group);
+  fb.init(wj, lane, group);
 
   f4 acc[MI][NI];
 #pragma unroll
@@ -323,7 +338,7 @@ __global__ __launch_bounds__(256, OCC) void k_dense(const GemmArgs a, const EpiD
   // from LDS into the other set.  A new stage's fragments are read after a barrier that says that its
   // loads have landed; the same barrier says that everyone has read the stage before it, whose buffer
   // then takes the stage ST later.  Stages past the end load zeros, so every stage has the same loads.
-  constexpr int BUF = SA::BYTES + SB::BYTES, LOADS = SA::LOADS + SB::LOADS, KS = KB / 64;
+  constexpr int BUF = SA::BYTES + SB::BYTES, LOADS = SA::LOADS + SB::LOADS, KS = KB / 64 / KG;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void*)smem + wave * 1024;
   typename FA::frag av[2][MI];
   typename FB::frag bv[2][NI];
@@ -415,6 +430,22 @@ __global__ __launch_bounds__(256, OCC) void k_dense(const GemmArgs a, const EpiD
   }
   wait_loads<0>();
   if constexpr (BIG) settle(acc);
+  if constexpr (KG > 1) {  // the second group's sums to the first
+    f4* const other = reinterpret_cast<f4*>(smem) + wpos * (MI * NI * 64) + lane;
+    __syncthreads();
+    if (group == 1) {
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) other[(i * NI + j) * 64] = acc[i][j];
+    }
+    __syncthreads();
+    if (group == 1) return;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) acc[i][j] += other[(i * NI + j) * 64];
+  }
 
   const int g = lane >> 4;
   if constexpr (PART) {
@@ -435,8 +466,8 @@ __global__ __launch_bounds__(256, OCC) void k_dense(const GemmArgs a, const EpiD
     typedef Turned<BM, BN, WM, WN> TU;
     constexpr int CR = TU::CR, PITCH = TU::PITCH, LPR = WN / 8, RPI = 64 / LPR, IT = CR / RPI;
     constexpr int U = BIG ? 4 : 2;
-    __syncthreads();  // the stages' LDS is free
-    float* const mine = reinterpret_cast<float*>(smem + wave * TU::BYTES);
+    if constexpr (KG == 1) __syncthreads();  // the stages' LDS is free
+    float* const mine = reinterpret_cast<float*>(smem + TU::at(wpos, KG > 1 ? 4 * MI * NI * 1024 : 0));
     const uint64_t sub = e.drop.thr ? drop_sub(e.drop) : 0;
     const int lr = lane / LPR;
     auto out = [&](auto chunk) __attribute__((always_inline)) {
@@ -496,20 +527,21 @@ inline void allow_lds(const void* fn, size_t bytes, std::atomic<uint64_t>& done)
   done.fetch_or(bit, std::memory_order_relaxed);
 }
 
-template <class T, bool AKC, bool BKC, int BM, int BN, int WM, int WN, int KB, int ST, int OCC>
+template <class T, bool AKC, bool BKC, int BM, int BN, int WM, int WN, int KB, int ST, int OCC, int KG = 1>
 hipError_t launch_tile(const GemmArgs& a, const EpiDev& e, hipStream_t s) {
-  const size_t lds = std::max(ST * (BM + BN) * KB, 4 * Turned<BM, BN, WM, WN>::BYTES);
+  constexpr int SUMS = KG > 1 ? BM * BN * 4 : 0;  // the second group's
+  const size_t lds = std::max(ST * (BM + BN) * KB, SUMS + 4 * Turned<BM, BN, WM, WN>::BYTES);
   const dim3 grid((unsigned)(a.n_mt * a.n_nt * a.splits));
   if (a.part) {
-    const auto fn = &k_dense<T, AKC, BKC, BM, BN, WM, WN, KB, ST, OCC, true>;
+    const auto fn = &k_dense<T, AKC, BKC, BM, BN, WM, WN, KB, ST, OCC, KG, true>;
     static std::atomic<uint64_t> done;
     allow_lds((const void*)fn, lds, done);
-    hipLaunchKernelGGL(fn, grid, dim3(256), lds, s, a, e);
+    hipLaunchKernelGGL(fn, grid, dim3(256 * KG), lds, s, a, e);
   } else {
-    const auto fn = &k_dense<T, AKC, BKC, BM, BN, WM, WN, KB, ST, OCC, false>;
+    const auto fn = &k_dense<T, AKC, BKC, BM, BN, WM, WN, KB, ST, OCC, KG, false>;
     static std::atomic<uint64_t> done;
     allow_lds((const void*)fn, lds, done);
-    hipLaunchKernelGGL(fn, grid, dim3(256), lds, s, a, e);
+    hipLaunchKernelGGL(fn, grid, dim3(256 * KG), lds, s, a, e);
   }
   return hipGetLastError();
 }
@@ -521,7 +553,7 @@ hipError_t launch_layout(int tile, const GemmArgs& a, const EpiDev& e, hipStream
     if (tile == TILE_256N) return launch_tile<T, AKC, BKC, 256, 128, 128, 64, 64, 3, 2>(a, e, s);
   }
   if (tile == TILE_128) return launch_tile<T, AKC, BKC, 128, 128, 64, 64, 64, 4, 2>(a, e, s);
-  if (tile == TILE_64) return launch_tile<T, AKC, BKC, 64, 64, 32, 32, 128, 3, 3>(a, e, s);
+  if (tile == TILE_64) return launch_tile<T, AKC, BKC, 64, 64, 32, 32, 128, 3, 3, sizeof(T) == 4 ? 2 : 1>(a, e, s);
   return launch_tile<T, AKC, BKC, 32, 128, 32, 32, 128, 4, 2>(a, e, s);
 }
 
