@@ -12,6 +12,14 @@ namespace {
 inline int64_t up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 inline int64_t cdiv(int64_t x, int64_t m) { return (x + m - 1) / m; }
 
+// A launch has fewer than 2^32 threads in a dimension; element-wise kernels of more workgroups than
+// kGridX have rows of them.
+constexpr int kGridX = 1 << 22;
+inline dim3 grid_of(int64_t blocks) {
+  return dim3((unsigned)std::min<int64_t>(blocks, kGridX), (unsigned)cdiv(blocks, kGridX));
+}
+__device__ __forceinline__ int64_t block_of() { return (int64_t)blockIdx.y * kGridX + blockIdx.x; }
+
 // ---------------------------------------------------------------- packing
 // Rows of `cols` elements at any stride and alignment to rows of a multiple of eight, zero-padded: the
 // tiled product reads 16 bytes at a time.  Two matrices a launch, so that a product with two odd operands
@@ -27,10 +35,11 @@ struct PackDev {
 template <class T>
 __global__ __launch_bounds__(256) void k_pack(const PackDev a, const PackDev b) {
   const int64_t na = a.blocks();
-  const bool first = blockIdx.x < na;
+  const int64_t at = block_of();
+  const bool first = at < na;
   const PackDev p = first ? a : b;
   const int per = p.per();
-  const int64_t q = (int64_t)(first ? blockIdx.x : blockIdx.x - na) * 256 + threadIdx.x;
+  const int64_t q = (first ? at : at - na) * 256 + threadIdx.x;
   if (q >= (int64_t)p.rows * per) return;
   const int64_t row = row_of(q, per);
   const int col = (int)(q - row * per) * 8;
@@ -341,7 +350,7 @@ __global__ __launch_bounds__(256) void k_dropout(const T* __restrict__ x, int64_
                                                  const T* __restrict__ res, int64_t ldr,
                                                  T* __restrict__ y, int64_t total, int groups, int n,
                                                  const DropDev d) {
-  const int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t q = block_of() * 256 + threadIdx.x;
   if (q >= total) return;
   const uint64_t sub = drop_sub(d);
   if constexpr (FLAT) {
@@ -377,6 +386,8 @@ struct Shape {
   int tile, n_mt, n_nt, splits, stages, stages_split;
 };
 constexpr int64_t kMaxWidth = 1 << 20;  // a tile's rows stay within a buffer descriptor's range
+constexpr int64_t kMaxM = ((int64_t)1 << 31) - 512;  // row numbers up to a tile's end, and of stages, fit 32 bits
+constexpr int64_t kMaxRow = ((int64_t)1 << 31) - 8;  // the end of a row's last group fits 32 bits
 
 // Tile and parts of K for an I x J result: the pair with the least estimated time.  A CU that gets c
 // workgroups takes  fixed + c (out + rate K / parts)  microseconds (K in units of 1024); joining P
@@ -398,7 +409,8 @@ Shape shape_of(int64_t I, int64_t J, int64_t K, int es) {
     const TileShape ts = kTiles[tile];
     const TileCost tc = es == 4 ? kCost32[tile] : kCost16[tile];
     const int64_t mt = cdiv(I, ts.bm), nt = cdiv(J, ts.bn), stages = cdiv(K * es, ts.kb);
-    if (mt * nt >= (int64_t)1 << 26) continue;  // workgroups of a launch, times 32 parts at most
+    // threads of a launch (check_dims leaves room for the 128 x 128 tile)
+    if (mt * nt * (tile == TILE_64 && es == 4 ? 512 : 256) >= (int64_t)1 << 32) continue;
     for (int64_t want = 1; want <= 32; want *= 2) {
       if (want > 1 && (stages < 4 * want || mt * nt > 1024)) break;
       const int64_t per = cdiv(stages, want), parts = cdiv(stages, per);
@@ -465,7 +477,7 @@ hipError_t pack(int dtype, const PackDev& a, const PackDev& b, hipStream_t s) {
   const int64_t blocks = a.blocks() + b.blocks();
   if (!blocks) return hipSuccess;
   return with_type(dtype, [&](auto* t) {
-    hipLaunchKernelGGL((k_pack<DENSE_T(t)>), dim3((unsigned)blocks), dim3(256), 0, s, a, b);
+    hipLaunchKernelGGL((k_pack<DENSE_T(t)>), grid_of(blocks), dim3(256), 0, s, a, b);
     return hipGetLastError();
   });
 }
@@ -546,13 +558,11 @@ int check_dims(int32_t dtype, int32_t act, int64_t m, int64_t k, int64_t n, int6
   if (dtype != DGPRF_F32 && dtype != DGPRF_F16 && dtype != DGPRF_BF16) return DGPRF_E_ARG;
   if (act < DGPRF_ACT_NONE || act > DGPRF_ACT_SILU) return DGPRF_E_ARG;
   if (m < 0 || k < 1 || n < 1 || ldx < k || ldw < n) return DGPRF_E_SHAPE;
-  if (m >= ((int64_t)1 << 31) || k > kMaxWidth || n > kMaxWidth || ldx > kMaxWidth || ldw > kMaxWidth)
+  if (m > kMaxM || k > kMaxWidth || n > kMaxWidth || ldx > kMaxWidth || ldw > kMaxWidth)
     return DGPRF_E_SHAPE;
-  // workgroups of a launch: of 256 groups of eight columns, and of 128 x 128 tiles
-  const int64_t w = std::max(k, n);
-  if (m * cdiv(w, 8) >= ((int64_t)1 << 39) || cdiv(m, 128) * cdiv(w, 128) >= ((int64_t)1 << 26) ||
-      cdiv(k, 128) * cdiv(n, 128) >= ((int64_t)1 << 26))
-    return DGPRF_E_SHAPE;
+  // 128 x 128 tiles of a launch: 2^38 elements
+  const int64_t w = std::max(k, n), most = (int64_t)1 << 24;
+  if (cdiv(m, 128) * cdiv(w, 128) >= most || cdiv(k, 128) * cdiv(n, 128) >= most) return DGPRF_E_SHAPE;
   return DGPRF_OK;
 }
 
@@ -662,11 +672,11 @@ hipError_t backward(const dgprf_linear_grad_t& a, Scratch& sc, hipStream_t st, b
 
 // zeros without a memset node (a captured graph replays a fill kernel)
 __global__ __launch_bounds__(256) void k_zero(uint16_t* p, int64_t n) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t i = block_of() * 256 + threadIdx.x;
   if (i < n) p[i] = 0;
 }
 hipError_t zero(void* p, int64_t bytes, hipStream_t s) {
-  hipLaunchKernelGGL(k_zero, dim3((unsigned)cdiv(bytes / 2, 256)), dim3(256), 0, s, (uint16_t*)p, bytes / 2);
+  hipLaunchKernelGGL(k_zero, grid_of(cdiv(bytes / 2, 256)), dim3(256), 0, s, (uint16_t*)p, bytes / 2);
   return hipGetLastError();
 }
 
@@ -748,7 +758,7 @@ int dgprf_dropout(int32_t dtype, const void* x, int64_t rows, int64_t n, int64_t
                   void* stream) {
   if (dtype != DGPRF_F32 && dtype != DGPRF_F16 && dtype != DGPRF_BF16) return DGPRF_E_ARG;
   if (check_drop(drop_thr)) return DGPRF_E_ARG;
-  if (rows < 0 || n < 0 || n >= ((int64_t)1 << 31) || (rows > 1 && ldx != 0 && ldx < n) || ldx < 0) return DGPRF_E_SHAPE;
+  if (rows < 0 || n < 0 || n > kMaxRow || (rows > 1 && ldx != 0 && ldx < n) || ldx < 0) return DGPRF_E_SHAPE;
   if (res && (ldr < 0 || (rows > 1 && ldr != 0 && ldr < n))) return DGPRF_E_SHAPE;
   if (rows == 0 || n == 0) return DGPRF_OK;
   if (!x || !y) return DGPRF_E_ARG;
@@ -760,7 +770,7 @@ int dgprf_dropout(int32_t dtype, const void* x, int64_t rows, int64_t n, int64_t
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   return hip_rc(with_type(dtype, [&](auto* t) {
     typedef DENSE_T(t) T;
-    const dim3 grid((unsigned)cdiv(total, 256));
+    const dim3 grid = grid_of(cdiv(total, 256));
     if (flat)
       hipLaunchKernelGGL((k_dropout<T, true>), grid, dim3(256), 0, s, (const T*)x, ldx, (const T*)res, ldr, (T*)y,
                          total, (int)groups, (int)n, d);

@@ -87,12 +87,12 @@ __device__ __forceinline__ float act_of(float z) {
   return z;
 }
 
-// a'(z).  z is clamped in the products that vanish for large |z|, so an infinite z has the limit
+// a'(z), of what saved_of() kept.  z is clamped in the products that vanish for large |z|, so an infinite z has the limit
 // (0 or 1) and not inf * 0.
 template <class T, int ACT>
 __device__ __forceinline__ float slope_of(float z) {
   const float zc = __builtin_amdgcn_fmed3f(z, -60.f, 60.f);
-  if constexpr (ACT == DGPRF_ACT_RELU) return z > 0.f ? 1.f : 0.f;
+  if constexpr (ACT == DGPRF_ACT_RELU) return z;  // as saved
   if constexpr (ACT == DGPRF_ACT_GELU) {
     const float tail = tail_of<T>(fabsf(z));
     return fmaf(zc * 0.3989422804014327f, gauss(z), z < 0.f ? tail : 1.f - tail);
@@ -123,10 +123,10 @@ __device__ __forceinline__ void with_act(int act, F f) {
 
 // What the backward pass needs of z, as it is stored.  Rounding z costs the slope less than the
 // rounding of dz itself costs (z a''(z) is below 0.4); relu's slope is stored instead, because a
-// small z could round to the other side of its jump.
+// small z could round to the other side of its jump (1 for a NaN, which relu passes on).
 template <int ACT>
 __device__ __forceinline__ float saved_of(float z) {
-  if constexpr (ACT == DGPRF_ACT_RELU) return z > 0.f ? 1.f : 0.f;
+  if constexpr (ACT == DGPRF_ACT_RELU) return z <= 0.f ? 0.f : 1.f;
   return z;
 }
 

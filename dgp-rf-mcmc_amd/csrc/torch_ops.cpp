@@ -266,6 +266,7 @@ Tensor rows_of(const Tensor& t, int64_t n) {
                   (m.size(0) <= 1 || m.stride(0) == 0 || m.stride(0) >= n);
   return ok ? m : m.contiguous();
 }
+constexpr int64_t kMaxStride = 1 << 20;  // of the operands of a product
 int64_t row_stride(const Tensor& t) { return t.size(0) <= 1 ? t.size(1) : t.stride(0); }
 // the same where rows may not share memory
 Tensor apart(const Tensor& t) { return t.size(0) > 1 && t.stride(0) < t.size(1) ? t.contiguous() : t; }
@@ -368,7 +369,8 @@ struct LinearFunction : public torch::autograd::Function<LinearFunction> {
     if (want_x || want_w || want_b) {
       const at::NoGradGuard no_grad;
       const c10::DeviceGuard guard(x.device());
-      const Tensor dy = rows_of(grads[0], w.size(1));
+      Tensor dy = rows_of(grads[0], w.size(1));
+      if (row_stride(dy) > kMaxStride) dy = dy.contiguous();
       dgprf_linear_grad_t a;
       std::memset(&a, 0, sizeof(a));
       a.dtype = dense_type(x, "x");

@@ -422,7 +422,8 @@ int dgprf_mass_estimate(const dgprf_plan_t *plan, const float *mean, const float
  * All tensors of a call have one element type (DGPRF_F32 / F16 / BF16) and unit stride within a row.
  * Sums, bias, activation, mask and residual are in 32 bits; a value is rounded once, where it is
  * stored.  16-bit backward passes round dz to the type before its two products.
- * Sizes: k, n and the row strides up to 2^20, m below 2^31; m = 0 is allowed. */
+ * Sizes: k, n and the row strides up to 2^20, m up to 2^31 - 512, results up to 2^38 elements; m = 0 is
+ * allowed. */
 #define DGPRF_F32 0
 #define DGPRF_F16 1
 #define DGPRF_BF16 2
@@ -479,7 +480,8 @@ int dgprf_linear_forward(const dgprf_linear_t *a, void *scratch, int64_t scratch
                          void *stream);
 int dgprf_linear_backward(const dgprf_linear_grad_t *a, void *scratch, int64_t scratch_bytes,
                           void *stream);
-/* y [rows][n] (rows without gaps) = res + s m x; its backward is the same call on dy without res. */
+/* y [rows][n] (rows without gaps) = res + s m x; its backward is the same call on dy without res.
+ * n up to 2^31 - 8, rows ceil(n / 8) up to 2^39. */
 int dgprf_dropout(int32_t dtype, const void *x, int64_t rows, int64_t n, int64_t ldx,
                   const void *res, int64_t ldr, int32_t drop_thr, uint64_t seed, uint64_t sub,
                   const int64_t *step, void *y, void *stream);

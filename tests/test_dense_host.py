@@ -62,6 +62,17 @@ def test_shapes_refused(make, bad):
     assert scratch(make(**bad))[0] == N.E_SHAPE
 
 
+def test_row_numbers_fit():
+    """Row numbers up to a tile's end fit 32 bits, and tiles a launch."""
+    for make in (linear, grad):
+        ones = dict(k=1, n=1, ldx=1, ldw=1)
+        assert scratch(make(m=2 ** 31 - 512, **ones))[0] == 0
+        assert scratch(make(m=2 ** 31 - 511, **ones))[0] == N.E_SHAPE
+        assert scratch(make(m=2 ** 31 - 512, k=1, n=256, ldx=1, ldw=256))[0] == N.E_SHAPE
+    some = 1 << 20  # never read
+    assert N.lib().dgprf_dropout(0, some, 1, 2 ** 31 - 7, 2 ** 31, None, 0, 1, 0, 0, None, some, None) == N.E_SHAPE
+
+
 def test_calls_refused_before_anything_is_enqueued():
     lib, e = N.lib(), ctypes.byref
     assert lib.dgprf_linear_forward(None, None, 0, None) == N.E_ARG

@@ -476,6 +476,47 @@ def test_offsets_past_32_bits():
     assert torch.equal(dw, (x[tail].float().t().contiguous() @ dz).to(t))
 
 
+def test_most_rows():
+    """As many rows as are allowed, and more groups than a launch has threads in a dimension."""
+    m, t = 2 ** 31 - 512, torch.float16
+    if torch.cuda.mem_get_info()[0] < 120 << 30:
+        pytest.skip("needs 120 GB")
+    x = torch.zeros(m, 1, dtype=t, device=DEV)
+    for first in (0, 2 ** 30 - 100, m - 200):
+        x[first:first + 200] = torch.arange(1, 201, dtype=t, device=DEV)[:, None]
+    w = torch.full((1, 1), 2.0, dtype=t, device=DEV, requires_grad=True)
+    y = dgprf.linear(x, w, residual=x)
+    assert torch.equal(y.detach()[m - 200:], 3 * x[m - 200:]) and torch.equal(y.detach()[2 ** 30 - 100:2 ** 30 + 100], 3 * x[:200])
+    assert not bool(y.detach()[200:2 ** 30 - 100].any()) and not bool(y.detach()[2 ** 30 + 100:m - 200].any())
+    dy = torch.zeros_like(x)
+    dy[m - 200:] = 0.5
+    dw, = torch.autograd.grad(y, w, dy)
+    assert float(dw) == float(torch.tensor(0.5 * 200 * 201 / 2).to(t))  # 10050: fp16's steps there are 8
+    del x, y, dy
+    rows = 2 ** 32 + 300
+    y = dgprf.dropout(torch.ones(1, 1, dtype=t, device=DEV).expand(rows, 1), 0.5, seed=3, sub=4)
+    for first in (0, 2 ** 30 - 100, 2 ** 32 - 100, rows - 200):
+        assert torch.equal(y[first:first + 200].cpu() != 0, keep_rows(first, 200, 1, 32768, 3, 4)), first
+
+
+def test_relu_passes_a_nan_on():
+    """z = NaN: the result is NaN, and the gradient goes through as for z > 0."""
+    for t in TYPES.values():
+        x, w = torch.ones(6, 8, dtype=t, device=DEV), torch.ones(8, 16, dtype=t, device=DEV)
+        x[2, 3] = float("nan")
+        x.requires_grad_()
+        y = dgprf.linear(x, w, activation="relu")
+        dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+        assert bool(torch.isnan(y[2]).all()) and bool((dx == 16).all())
+
+
+def test_gradient_of_rows_far_apart():
+    x, w = torch.ones(3, 8, device=DEV, requires_grad=True), torch.ones(8, 16, device=DEV, requires_grad=True)
+    dy = torch.ones(3, (1 << 20) + 16, device=DEV)[:, :16]
+    dx, dw = torch.autograd.grad(dgprf.linear(x, w), (x, w), dy)
+    assert bool((dx == 16).all()) and bool((dw == 3).all())
+
+
 def keep_rows(first, rows, n, thr, seed, sub):
     """keep_mask's rows first .. first + rows - 1 (groups numbered from row 0)."""
     from oracle import rng
