@@ -25,6 +25,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
@@ -346,6 +347,29 @@ variable_list once(variable_list grads, const char* what) {
   return (*error)(std::move(grads));
 }
 
+bool capturing(hipStream_t s) {  // (the null stream cannot be captured, and must not be asked while another is)
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  return s && hipStreamIsCapturing(s, &status) == hipSuccess && status == hipStreamCaptureStatusActive;
+}
+// A leaf that an earlier, living autograd graph uses has its accumulation on that graph's stream.  The
+// engine would make that stream wait for the captured one, which ends the capture and then the process;
+// called in a backward pass, before anything is enqueued.
+void check_capture(const char* what) {
+  if (!capturing(c10::hip::getCurrentHIPStream().stream())) return;
+  const auto node = torch::autograd::get_current_node();
+  if (!node) return;
+  for (size_t i = 0; i < node->num_outputs(); ++i) {
+    const auto& next = node->next_edge(i).function;
+    if (!node->task_should_compute_output(i) || !dynamic_cast<torch::autograd::AccumulateGrad*>(next.get())) continue;
+    const auto s = next->stream();
+    if (!s) continue;
+    const c10::Stream h(c10::Stream::UNSAFE, c10::Device(c10::DeviceType::HIP, s->device_index()), s->id());
+    TORCH_CHECK(capturing(c10::hip::HIPStream(c10::hip::HIPStream::UNCHECKED, h).stream()), "dgprf: ", what,
+                ": this backward pass is being captured while an autograd graph from before the capture holds one "
+                "of its leaves; delete that graph's results first");
+  }
+}
+
 struct LinearFunction : public torch::autograd::Function<LinearFunction> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptT& bias,
                         const OptT& res, int64_t act, int64_t thr, int64_t seed, int64_t sub, const OptT& step) {
@@ -365,10 +389,11 @@ struct LinearFunction : public torch::autograd::Function<LinearFunction> {
     const bool bias = args[4], res = args[5];
     const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
     const bool want_b = bias && ctx->needs_input_grad(2), want_r = res && ctx->needs_input_grad(bias ? 3 : 2);
+    const c10::DeviceGuard guard(x.device());
+    check_capture("linear");
     Tensor dx, dw, db;
     if (want_x || want_w || want_b) {
       const at::NoGradGuard no_grad;
-      const c10::DeviceGuard guard(x.device());
       Tensor dy = rows_of(grads[0], w.size(1));
       if (row_stride(dy) > kMaxStride) dy = dy.contiguous();
       dgprf_linear_grad_t a;
@@ -414,6 +439,8 @@ struct DropoutFunction : public torch::autograd::Function<DropoutFunction> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const Tensor step = ctx->get_saved_variables()[0];
     const auto args = ctx->saved_data["args"].toIntVector();
+    const c10::DeviceGuard guard(grads[0].device());
+    check_capture("dropout");
     Tensor dx;
     if (ctx->needs_input_grad(0)) {
       const at::NoGradGuard no_grad;

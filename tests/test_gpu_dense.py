@@ -355,6 +355,32 @@ def test_captured_training_step():
         assert int(step) == i + 1
 
 
+def test_capture_beside_an_eager_graph():
+    """A backward pass captured while an eager graph of the same leaves lives is refused, before anything
+    is enqueued; once that graph is gone, the same capture works."""
+    x, w = torch.ones(4, 8, device=DEV, requires_grad=True), torch.ones(8, 16, device=DEV, requires_grad=True)
+    dy = torch.ones(4, 16, device=DEV)
+    for op in (lambda: dgprf.linear(x, w, activation="relu"), lambda: dgprf.dropout(dgprf.linear(x, w), 0.0),
+               lambda: dgprf.linear(dgprf.dropout(x, 0.0), w),
+               lambda: dgprf.dropout(dgprf.linear(x, w).detach(), 0.0, residual=dgprf.linear(x, w))):
+        held = op()
+        with pytest.raises(RuntimeError, match="being captured"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                y = op()
+                torch.autograd.grad(y, (x, w), dy)
+        assert torch.equal(torch.autograd.grad(held, w, dy)[0], torch.full_like(w, 4))
+        del held, y
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = op()
+            dx, dw = torch.autograd.grad(y, (x, w), dy)
+        for _ in range(2):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert bool((dx == 16).all()) and bool((dw == 4).all())
+        del y
+
+
 def test_two_graphs_and_streams():
     """Two captured calls do not share scratch, and a call on another stream is ordered there."""
     g = _gen(8)
