@@ -392,15 +392,18 @@ constexpr int64_t kMaxRow = ((int64_t)1 << 31) - 8;  // the end of a row's last 
 // Tile and parts of K for an I x J result: the pair with the least estimated time.  A CU that gets c
 // workgroups takes  fixed + c (out + rate K / parts)  microseconds (K in units of 1024); joining P
 // parts costs a launch and P I J 8 bytes of traffic at 5.5 TB/s.  The three numbers of a tile come from
-// runs with one to four workgroups per CU at K = 512 .. 8192 (4096 x 2048 x 4096 in bf16: 60 us with
-// 256 x 256 tiles, 68 with 256 x 128, 76 with 128 x 128; 2048 x 2048 x 2048: 47, 32, 23, and 30 with
-// 64 x 64; 64 x 4096 x 4096: 12.4 with 32 x 128 and four parts, 19 with one).
+// runs with one to four workgroups per CU at K = 512 .. 8192 (2048 x 2048 x 2048 in bf16: 47 us with
+// 256 x 256 tiles, 32 with 256 x 128, 23 with 128 x 128, 30 with 64 x 64; 64 x 4096 x 4096: 12.4 with
+// 32 x 128 and four parts, 19 with one).  Tiles with two groups of waves are for launches of at most one
+// workgroup a CU: nothing runs beside a workgroup's last rows (256 x 128, 4096 x 2048 over K = 8192: 109 us,
+// 126 with one group; 8192 x 8192 over 1024: 164 and 131).
 struct TileCost {
   float fixed, out, rate;
 };
-constexpr TileCost kCost16[TILES] = {{3.f, 12.f, 22.5f}, {9.f, 1.f, 14.4f}, {5.f, 0.5f, 9.2f}, {4.5f, 0.5f, 3.3f}, {4.f, 0.5f, 3.4f}};
+constexpr TileCost kCost16[TILES] = {{3.f, 12.f, 22.5f}, {9.f, 1.f, 14.4f}, {6.f, 0.f, 13.f},  {7.6f, 0.f, 7.f},
+                                     {5.f, 0.5f, 9.2f},  {4.5f, 0.5f, 3.3f}, {4.f, 0.5f, 3.4f}};
 // fp32: 65 us of 4096 multiply-adds a clock; the 256-wide tiles' accumulators and fragments do not fit
-constexpr TileCost kCost32[TILES] = {{0, 0, 0}, {0, 0, 0}, {5.f, 1.f, 59.f}, {5.f, 0.5f, 17.f}, {5.f, 0.5f, 17.5f}};
+constexpr TileCost kCost32[TILES] = {{}, {}, {}, {}, {5.f, 1.f, 59.f}, {5.f, 0.5f, 17.f}, {5.f, 0.5f, 17.5f}};
 
 Shape shape_of(int64_t I, int64_t J, int64_t K, int es) {
   Shape best{};
@@ -410,10 +413,11 @@ Shape shape_of(int64_t I, int64_t J, int64_t K, int es) {
     const TileCost tc = es == 4 ? kCost32[tile] : kCost16[tile];
     const int64_t mt = cdiv(I, ts.bm), nt = cdiv(J, ts.bn), stages = cdiv(K * es, ts.kb);
     // threads of a launch (check_dims leaves room for the 128 x 128 tile)
-    if (mt * nt * (tile == TILE_64 && es == 4 ? 512 : 256) >= (int64_t)1 << 32) continue;
+    if (mt * nt * ts.threads >= (int64_t)1 << 32) continue;
     for (int64_t want = 1; want <= 32; want *= 2) {
       if (want > 1 && (stages < 4 * want || mt * nt > 1024)) break;
       const int64_t per = cdiv(stages, want), parts = cdiv(stages, per);
+      if ((tile == TILE_256G || tile == TILE_128G) && mt * nt * parts > 256) break;
       const float k = (float)per * ts.kb / es / 1024.f, rounds = (float)cdiv(mt * nt * parts, 256);
       float t = tc.fixed + rounds * (tc.out + tc.rate * k);
       if (parts > 1) t += 4.f + (float)parts * I * J * 8.f / 5.5e6f;

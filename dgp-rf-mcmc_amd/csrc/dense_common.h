@@ -318,11 +318,13 @@ struct GemmArgs {
 };
 
 enum { LAYOUT_NN = 0, LAYOUT_NT = 1, LAYOUT_TN = 2 };  // forward, dx, dW
-enum { TILE_256 = 0, TILE_256N = 1, TILE_128 = 2, TILE_64 = 3, TILE_32 = 4, TILES = 5 };
+// G: two groups of waves; those before TILE_128 are for 16-bit types
+enum { TILE_256 = 0, TILE_256N, TILE_256G, TILE_128G, TILE_128, TILE_64, TILE_32, TILES };
 struct TileShape {
-  int bm, bn, kb;  // rows, columns, bytes of K of a stage
+  int bm, bn, kb, threads;  // rows, columns, bytes of K of a stage, threads at most
 };
-constexpr TileShape kTiles[TILES] = {{256, 256, 128}, {256, 128, 64}, {128, 128, 64}, {64, 64, 128}, {32, 128, 128}};
+constexpr TileShape kTiles[TILES] = {{256, 256, 128, 256}, {256, 128, 64, 256}, {256, 128, 128, 512}, {128, 128, 128, 512},
+                                     {128, 128, 64, 256},  {64, 64, 128, 512}, {32, 128, 128, 256}};
 
 // one instantiation per element type (dense_<type>.hip): layout, tile, and epilogue (part == null:
 // the linear epilogue e; otherwise partial sums)

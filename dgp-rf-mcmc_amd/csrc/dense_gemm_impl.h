@@ -2,7 +2,7 @@
 // products of a layer: forward z = x W (A[i][k], B[k][j]), dx = dz W^T (A[i][k], B[j][k]) and
 // dW = x^T dz (A[k][i], B[k][j]); x, W and dz stay in their row-major layouts.
 //
-// A workgroup of four waves computes a BM x BN tile; a stage is KB bytes of K (64 or 128; 64 bytes
+// A workgroup of four waves, or two groups of four, computes a BM x BN tile; a stage is KB bytes of K (64 or 128; 64 bytes
 // are 32 16-bit or 16 fp32 elements, one step of the matrix instructions).  Both operands' stages go
 // from memory to LDS without passing registers (16-byte buffer loads with the LDS destination) into
 // ST buffers, one barrier per stage.  The LDS image of a load is linear in the lane, so bank conflicts
@@ -25,9 +25,13 @@
 //    product of the type reaches 1.26; bound by the matrix instructions at the clock that they allow.
 //  * 256 x 128 (16-bit) and 128 x 128: two workgroups a CU, one's epilogue beside the other's product;
 //    bound by LDS.
-//  * 64 x 64: for results of few tiles.  fp32 takes two groups of four waves, one for each step of a
-//    stage, whose sums are added at the end (1024 x 2048 x 1024: 40 us, 43 with one); 16-bit steps are
-//    too short for that (1024 x 2048 x 2048 in bf16: 19 us, 16 with one).
+//  * The same with two groups of four waves (16-bit), one for each step of a stage: where a CU gets one
+//    workgroup, a second wave on each SIMD runs while the first waits, for the same bytes from LDS (eight
+//    smaller sub-tiles would take more).  At the end each group takes the other's sums of half of the
+//    rows and finishes those.  4096 x 2048 over K = 8192 in bf16: 109 us with 256 x 128, 126 with one group;
+//    2048 x 2048 x 2048: 20.9 with 128 x 128, 22.8.
+//  * 64 x 64: for results of few tiles.  fp32 takes two groups (1024 x 2048 x 1024: 40 us, 43 with one);
+//    16-bit steps are too short for that (1024 x 2048 x 2048 in bf16: 19 us, 16 with one).
 //  * 32 x 128: for few rows; bound by the memory's rate (24 x 8192 x 2048 in fp16: 6.8 us, 4.9 TB/s).
 #pragma once
 
@@ -260,12 +264,11 @@ __device__ __forceinline__ void settle(f4 (&acc)[MI][NI]) {
     for (int j = 0; j < NI; ++j) asm volatile("" : "+a"(acc[i][j]));
 }
 
-// LDS that a wave's sub-tile takes on its way out, CR rows at a time; the pitch spreads the rows of a
-// write over the banks
-template <int BM, int BN, int WM, int WN>
+// LDS that a wave's rows take on their way out, CR at a time (a wave of two groups finishes half of its
+// sub-tile's); the pitch spreads the rows of a write over the banks
+template <int WM, int WN, int KG>
 struct Turned {
-  static constexpr int CR = WM < 64 ? WM : 64, PITCH = WN + 4, BYTES = CR * PITCH * 4;
-  __device__ static int at(int wave, int from) { return from + wave * BYTES; }  // `from`: sums of the second group
+  static constexpr int ROWS = WM / KG, CR = ROWS < 64 ? ROWS : 64, PITCH = WN + 4, BYTES = CR * PITCH * 4;
 };
 // the wave's LDS accesses before are done before those after
 __device__ __forceinline__ void wave_sync() {
@@ -284,8 +287,8 @@ template <class T, bool AKC, bool BKC, int BM, int BN, int WM, int WN, int KB, i
 __global__ __launch_bounds__(256 * KG, OCC) void k_dense(const GemmArgs a, const EpiDev e) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host pass needs the stub alone
   constexpr int NT = 256 * KG, MI = WM / 16, NI = WN / 16;
-  static_assert(BM / WM * (BN / WN) == 4, "four waves");
-  static_assert(KG == 1 || KG == KB / 64, "a group of waves for each step of a stage");
+  static_assert(BM / WM * (BN / WN) == 4, "four waves of a group");
+  static_assert(KG == 1 || (KG == 2 && KB == 128), "a group of waves for each step of a stage");
   constexpr bool BIG = MI * NI == 64;  // accumulators fill a register file
   static_assert(!BIG || (MI == 8 && NI == 8 && sizeof(T) == 2 && BM == 256), "turn()'s groups");
   typedef Stage<T, AKC, BM, KB, NT> SA;
@@ -430,44 +433,57 @@ __global__ __launch_bounds__(256 * KG, OCC) void k_dense(const GemmArgs a, const
   }
   wait_loads<0>();
   if constexpr (BIG) settle(acc);
-  if constexpr (KG > 1) {  // the second group's sums to the first
-    f4* const other = reinterpret_cast<f4*>(smem) + wpos * (MI * NI * 64) + lane;
+  // Two groups: each takes the other's sums of the half of the rows that it finishes.
+  constexpr int MF = MI / KG;
+  f4 half[MF][NI];
+  f4 (&fin)[MF][NI] = KG == 1 ? reinterpret_cast<f4 (&)[MF][NI]>(acc) : half;
+  if constexpr (KG > 1) {
+    f4* const give = reinterpret_cast<f4*>(smem) + wave * (MF * NI * 64) + lane;
+    const f4* const take = reinterpret_cast<f4*>(smem) + (wave ^ 4) * (MF * NI * 64) + lane;
+    auto put = [&](auto from) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < MF; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) give[(i * NI + j) * 64] = acc[decltype(from)::value + i][j];
+    };
+    auto sum = [&](auto from) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < MF; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) half[i][j] = acc[decltype(from)::value + i][j] + take[(i * NI + j) * 64];
+    };
+    typedef std::integral_constant<int, 0> First;
+    typedef std::integral_constant<int, MF> Second;
     __syncthreads();
-    if (group == 1) {
-#pragma unroll
-      for (int i = 0; i < MI; ++i)
-#pragma unroll
-        for (int j = 0; j < NI; ++j) other[(i * NI + j) * 64] = acc[i][j];
-    }
+    if (group == 0) put(Second());
+    else put(First());
     __syncthreads();
-    if (group == 1) return;
-#pragma unroll
-    for (int i = 0; i < MI; ++i)
-#pragma unroll
-      for (int j = 0; j < NI; ++j) acc[i][j] += other[(i * NI + j) * 64];
+    if (group == 0) sum(First());
+    else sum(Second());
   }
+  const int wr = i0 + wi + group * (WM / KG);  // the first row that this wave finishes
 
   const int g = lane >> 4;
   if constexpr (PART) {
-    const int r0 = i0 + wi + (lane & 15), c0 = j0 + wj + 4 * g;
+    const int r0 = wr + (lane & 15), c0 = j0 + wj + 4 * g;
     float* const out = a.part + (int64_t)split * a.I * a.ldp;
 #pragma unroll
-    for (int i = 0; i < MI; ++i)
+    for (int i = 0; i < MF; ++i)
 #pragma unroll
       for (int j = 0; j < NI; ++j) {
         const int row = r0 + 16 * i, col = c0 + 16 * j;
-        if (row < a.I && col < a.ldp) *reinterpret_cast<f4*>(out + (int64_t)row * a.ldp + col) = acc[i][j];
+        if (row < a.I && col < a.ldp) *reinterpret_cast<f4*>(out + (int64_t)row * a.ldp + col) = fin[i][j];
       }
   } else {
     // The wave's sub-tile goes through its own part of LDS, CR rows at a time, so that a lane gets eight
     // columns of a row (one generator call, one 16-byte access) and neighbouring lanes the row's next
     // ones: rows of 16 lanes' accesses instead of pieces of 32 bytes, and a loop instead of a body for
     // every accumulator.  U row groups at a time have their residual loads in flight together.
-    typedef Turned<BM, BN, WM, WN> TU;
+    typedef Turned<WM, WN, KG> TU;
     constexpr int CR = TU::CR, PITCH = TU::PITCH, LPR = WN / 8, RPI = 64 / LPR, IT = CR / RPI;
-    constexpr int U = BIG ? 4 : 2;
-    if constexpr (KG == 1) __syncthreads();  // the stages' LDS is free
-    float* const mine = reinterpret_cast<float*>(smem + TU::at(wpos, KG > 1 ? 4 * MI * NI * 1024 : 0));
+    constexpr int U = BIG ? 4 : IT < 2 ? 1 : 2;
+    __syncthreads();  // the LDS of the stages, and of the sums, is free
+    float* const mine = reinterpret_cast<float*>(smem + wave * TU::BYTES);
     const uint64_t sub = e.drop.thr ? drop_sub(e.drop) : 0;
     const int lr = lane / LPR;
     auto out = [&](auto chunk) __attribute__((always_inline)) {
@@ -476,13 +492,13 @@ __global__ __launch_bounds__(256 * KG, OCC) void k_dense(const GemmArgs a, const
       for (int i = 0; i < CR / 16; ++i)
 #pragma unroll
         for (int j = 0; j < NI; ++j)
-          *reinterpret_cast<f4*>(&mine[(16 * i + (lane & 15)) * PITCH + 16 * j + 4 * g]) = acc[CH * (CR / 16) + i][j];
+          *reinterpret_cast<f4*>(&mine[(16 * i + (lane & 15)) * PITCH + 16 * j + 4 * g]) = fin[CH * (CR / 16) + i][j];
       wave_sync();
       if (col < e.n) {
 #pragma unroll 1
         for (int it = 0; it < IT; it += U) {
           F8 res[U], v[U];
-          const int r = it * RPI + lr, row = i0 + wi + CH * CR + r;
+          const int r = it * RPI + lr, row = wr + CH * CR + r;
 #pragma unroll
           for (int u = 0; u < U; ++u) {
             if (e.res && row + u * RPI < a.I) res[u] = load8((const T*)e.res + (int64_t)(row + u * RPI) * e.ldr, col, e.n);
@@ -510,8 +526,8 @@ __global__ __launch_bounds__(256 * KG, OCC) void k_dense(const GemmArgs a, const
       wave_sync();
     };
     out(std::integral_constant<int, 0>());
-    if constexpr (WM / CR == 2) out(std::integral_constant<int, 1>());
-    static_assert(WM / CR <= 2, "chunks of a wave's rows");
+    if constexpr (TU::ROWS / CR == 2) out(std::integral_constant<int, 1>());
+    static_assert(TU::ROWS / CR <= 2, "chunks of a wave's rows");
   }
 #endif
 }
@@ -529,8 +545,9 @@ inline void allow_lds(const void* fn, size_t bytes, std::atomic<uint64_t>& done)
 
 template <class T, bool AKC, bool BKC, int BM, int BN, int WM, int WN, int KB, int ST, int OCC, int KG = 1>
 hipError_t launch_tile(const GemmArgs& a, const EpiDev& e, hipStream_t s) {
-  constexpr int SUMS = KG > 1 ? BM * BN * 4 : 0;  // the second group's
-  const size_t lds = std::max(ST * (BM + BN) * KB, SUMS + 4 * Turned<BM, BN, WM, WN>::BYTES);
+  constexpr int SUMS = KG > 1 ? BM * BN * 4 : 0;  // of two groups
+  constexpr size_t lds = std::max({ST * (BM + BN) * KB, SUMS, 4 * KG * Turned<WM, WN, KG>::BYTES});
+  static_assert(lds <= 160 * 1024, "LDS of a CU");
   const dim3 grid((unsigned)(a.n_mt * a.n_nt * a.splits));
   if (a.part) {
     const auto fn = &k_dense<T, AKC, BKC, BM, BN, WM, WN, KB, ST, OCC, KG, true>;
@@ -551,6 +568,8 @@ hipError_t launch_layout(int tile, const GemmArgs& a, const EpiDev& e, hipStream
   if constexpr (sizeof(T) == 2) {
     if (tile == TILE_256) return launch_tile<T, AKC, BKC, 256, 256, 128, 128, 128, 2, 1>(a, e, s);
     if (tile == TILE_256N) return launch_tile<T, AKC, BKC, 256, 128, 128, 64, 64, 3, 2>(a, e, s);
+    if (tile == TILE_256G) return launch_tile<T, AKC, BKC, 256, 128, 128, 64, 128, 3, 2, 2>(a, e, s);
+    if (tile == TILE_128G) return launch_tile<T, AKC, BKC, 128, 128, 64, 64, 128, 3, 2, 2>(a, e, s);
   }
   if (tile == TILE_128) return launch_tile<T, AKC, BKC, 128, 128, 64, 64, 64, 4, 2>(a, e, s);
   if (tile == TILE_64) return launch_tile<T, AKC, BKC, 64, 64, 32, 32, 128, 3, 3, sizeof(T) == 4 ? 2 : 1>(a, e, s);

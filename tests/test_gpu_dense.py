@@ -65,6 +65,25 @@ def test_products_exact(size, tname):
         assert got.dtype == t and torch.equal(got.cpu(), want.to(t).cpu()), name
 
 
+@pytest.mark.parametrize("tname", ["fp16", "bf16"])
+@pytest.mark.parametrize("size", [(2000, 1030, 1999), (1777, 1008, 2056), (2048, 8192, 1024), (2040, 2050, 4000),
+                                  (2500, 1999, 2500)], ids=str)
+def test_products_of_one_tile_a_cu(size, tname):
+    """Results of up to 256 tiles and longer K, whole and in parts: whole numbers again, with a bias, a
+    residual, relu and a mask in the epilogue."""
+    m, k, n = size
+    t, g = TYPES[tname], _gen(m + k + n)
+    x, w, b, r, dy = grid(g, m, k, t=t), grid(g, k, n, t=t), grid(g, n, t=t), grid(g, m, n, t=t), grid(g, m, n, t=t)
+    keep = 2 * keep_mask(m, n, 32768, 7, 8).to(DEV).float()
+    d = lambda v: v.to(DEV).float()  # noqa: E731
+    z = d(x) @ d(w) + d(b)
+    dz = d(dy) * keep * (z > 0)
+    y, dx, dw, db, dr = run(x, w, b, "relu", r, 0.5, 7, 8, dy)
+    for name, got, want in (("y", y, keep * z.clamp(min=0) + d(r)), ("dx", dx, dz @ d(w).t().contiguous()),
+                            ("dw", dw, d(x).t().contiguous() @ dz), ("db", db, dz.sum(0)), ("dr", dr, d(dy))):
+        assert got.dtype == t and torch.equal(got, want.to(t)), name
+
+
 @pytest.mark.parametrize("tname", TYPES)
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("size", [(1, 300, 200), (6, 65, 77), (40, 256, 136), (200, 784, 300), (130, 515, 261)], ids=str)
