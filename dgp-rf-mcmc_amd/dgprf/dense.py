@@ -18,15 +18,16 @@ def drop_threshold(p):
     return int(p * 65536 + 0.5)
 
 
-def _stream_of(thr, seed, sub):
+def _stream_of(thr, seed, sub, step):
     """(seed, sub) of this call's mask: as given, or the global generator's key and its next
-    subsequence (dgprf.set_seed makes a run's masks repeat)."""
+    subsequence (dgprf.set_seed makes a run's masks repeat).  With a step, the call has 2^32 of them to
+    itself: step is added to sub, and no other call's masks may come up."""
     if thr == 0:
         return 0, 0
     if seed is None:
         seed = E._RNG.seed
     if sub is None:
-        sub = E.next_subsequence()
+        sub = E.next_subsequence() if step is None else (E.next_subsequence() + 1) << 32
     return E._i64(seed), E._i64(sub)
 
 
@@ -39,13 +40,14 @@ def linear(x, weight, bias=None, activation="none", residual=None, dropout=0.0, 
     dropout: the probability p of an element's being dropped, rounded to a multiple of 1 / 65536.
     seed / sub: key and number of the mask (default: the global generator, its next subsequence);
     step: an int64 device tensor added to sub when the kernels run, for a captured call — advance it
-    after the call's backward pass.  The gradient of the gradient is not available.
+    after the call's backward pass, and keep given subs of different calls more than the number of
+    steps apart.  The gradient of the gradient is not available.
     """
     act = N.ACTS.get(activation)
     if act is None:
         raise ValueError(f"activation must be one of {', '.join(N.ACTS)}, got {activation!r}")
     thr = drop_threshold(dropout) if dropout else 0
-    seed, sub = _stream_of(thr, seed, sub)
+    seed, sub = _stream_of(thr, seed, sub, step)
     return E.ops().linear(x, weight, bias, act, residual, thr, seed, sub, step)
 
 
@@ -53,5 +55,5 @@ def dropout(x, p, residual=None, seed=None, sub=None, step=None):
     """y = residual + s m x for x [..., n]: the mask of `linear`'s result of the same rows, (seed, sub)
     and n.  p = 1 drops everything.  Arguments as in `linear`."""
     thr = drop_threshold(p)
-    seed, sub = _stream_of(thr, seed, sub)
+    seed, sub = _stream_of(thr, seed, sub, step)
     return E.ops().dropout(x, residual, thr, seed, sub, step)

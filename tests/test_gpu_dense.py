@@ -303,6 +303,19 @@ def test_masks_come_from_the_global_generator():
     assert torch.equal(dgprf.dropout(x, 0.5, seed=1, sub=2, step=step), dgprf.dropout(x, 0.5, seed=1, sub=7))
 
 
+def test_steps_of_calls_do_not_meet():
+    """With a step and the default numbers, no mask of one call comes up in another, whatever the steps."""
+    x, masks = torch.ones(64, 64, device=DEV), []
+    dgprf.set_seed(11)
+    step = torch.zeros(1, dtype=torch.int64, device=DEV)
+    for i in range(4):
+        dgprf.set_seed(11)
+        step.fill_(i)
+        masks += [dgprf.dropout(x, 0.5, step=step), dgprf.linear(x, torch.eye(64, device=DEV), dropout=0.5, step=step)]
+        masks += [dgprf.dropout(x, 0.5)] if i == 0 else []
+    assert len({m.cpu().numpy().tobytes() for m in masks}) == len(masks)
+
+
 def _block(x, w1, b1, w2, b2, step=None):
     """The operators as a network uses them: up-projection, dropout, down-projection onto the residual."""
     h = dgprf.linear(x, w1, b1, "gelu", dropout=0.2, seed=8, sub=0, step=step)
