@@ -557,6 +557,21 @@ def test_most_rows():
         assert torch.equal(y[first:first + 200].cpu() != 0, keep_rows(first, 200, 1, 32768, 3, 4)), first
 
 
+@pytest.mark.parametrize("tname", TYPES)
+@pytest.mark.parametrize("size", [(1, 2 ** 20, 16), (2, 2 ** 20, 9), (3, 2 ** 20 - 1, 8), (40, 2 ** 20, 8), (1, 8, 2 ** 20),
+                                  (16, 24, 2 ** 20), (300, 3, 2 ** 20 - 1)], ids=str)
+def test_widest(size, tname):
+    """The longest sums and rows that are allowed: whole numbers, whose sums here stay below 2^22."""
+    m, k, n = size
+    t, g = TYPES[tname], _gen(m + k + n)
+    x, w, b, dy = grid(g, m, k, t=t), grid(g, k, n, t=t), grid(g, n, t=t), grid(g, m, n, t=t)
+    y, dx, dw, db, _ = run(x, w, b, dy=dy)
+    d = lambda v: v.to(DEV).float()  # noqa: E731
+    for name, got, want in (("y", y, d(x) @ d(w) + d(b)), ("dx", dx, d(dy) @ d(w).t().contiguous()),
+                            ("dw", dw, d(x).t().contiguous() @ d(dy)), ("db", db, d(dy).sum(0))):
+        assert got.dtype == t and torch.equal(got, want.to(t)), name
+
+
 def test_relu_passes_a_nan_on():
     """z = NaN: the result is NaN, and the gradient goes through as for z > 0."""
     for t in TYPES.values():
