@@ -405,12 +405,14 @@ constexpr TileCost kCost16[TILES] = {{3.f, 12.f, 22.5f}, {9.f, 1.f, 14.4f}, {6.f
 // fp32: 65 us of 4096 multiply-adds a clock; the 256-wide tiles' accumulators and fragments do not fit
 constexpr TileCost kCost32[TILES] = {{}, {}, {}, {}, {5.f, 1.f, 59.f}, {5.f, 0.5f, 17.f}, {5.f, 0.5f, 17.5f}};
 
-Shape shape_of(int64_t I, int64_t J, int64_t K, int es) {
+Shape shape_of(int64_t I, int64_t J, int64_t K, int es, int layout) {
   Shape best{};
   float least = INFINITY;
   for (int tile = es == 4 ? TILE_128 : TILE_256; tile < TILES; ++tile) {
     const TileShape ts = kTiles[tile];
-    const TileCost tc = es == 4 ? kCost32[tile] : kCost16[tile];
+    TileCost tc = es == 4 ? kCost32[tile] : kCost16[tile];
+    // both operands read as whole fragments (1777 x 1008 over 2048: 15.6 us, 19.1 with 32 x 128)
+    if (es == 2 && tile == TILE_64 && layout == LAYOUT_NT) tc.rate *= 0.9f;
     const int64_t mt = cdiv(I, ts.bm), nt = cdiv(J, ts.bn), stages = cdiv(K * es, ts.kb);
     // threads of a launch (check_dims leaves room for the 128 x 128 tile)
     if (mt * nt * ts.threads >= (int64_t)1 << 32) continue;
@@ -521,7 +523,7 @@ hipError_t product(int dtype, int layout, const void* A, int64_t lda, const void
                    int64_t J, int64_t Ia, int64_t Ja, int64_t Ka, int64_t Kb, const EpiDev& e, Scratch& sc,
                    hipStream_t st, bool run) {
   const int es = elem_size(dtype);
-  const Shape s = shape_of(I, J, std::max(Ka, Kb), es);
+  const Shape s = shape_of(I, J, std::max(Ka, Kb), es, layout);
   float* part = (float*)sc.take(part_bytes(s, I, J));
   if (!run) return hipSuccess;
   GemmArgs a;
