@@ -84,6 +84,19 @@ def test_products_of_one_tile_a_cu(size, tname):
         assert got.dtype == t and torch.equal(got, want.to(t)), name
 
 
+@pytest.mark.parametrize("tname", ["fp16", "bf16"])
+@pytest.mark.parametrize("size", [(783, 5958, 268), (1227, 4998, 785), (1570, 14992, 2436), (2306, 15230, 1788)], ids=str)
+def test_large_tiles_in_parts_of_k(size, tname):
+    """Long sums of results with few large tiles: whole numbers again, a mask after the join."""
+    m, k, n = size
+    g = torch.Generator(device=DEV)
+    g.manual_seed(m)
+    draw = lambda *s: torch.randint(-2, 3, s, generator=g, device=DEV).to(TYPES[tname])  # noqa: E731
+    x, w, b, r = draw(m, k), draw(k, n), draw(n), draw(m, n)
+    want = 2 * keep_mask(m, n, 32768, 7, 8).to(DEV) * (x.float() @ w.float() + b.float()).clamp(min=0) + r.float()
+    assert torch.equal(dgprf.linear(x, w, b, "relu", r, 0.5, 7, 8), want.to(x.dtype))
+
+
 @pytest.mark.parametrize("tname", TYPES)
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("size", [(1, 300, 200), (6, 65, 77), (40, 256, 136), (200, 784, 300), (130, 515, 261)], ids=str)
