@@ -17,6 +17,7 @@
 #include <cmath>
 #include <cstring>
 #include <string>
+#include <unordered_set>
 #include <vector>
 
 #include <ATen/ops/add.h>
@@ -25,7 +26,6 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
@@ -351,22 +351,30 @@ bool capturing(hipStream_t s) {  // (the null stream cannot be captured, and mus
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
   return s && hipStreamIsCapturing(s, &status) == hipSuccess && status == hipStreamCaptureStatusActive;
 }
-// A leaf that an earlier, living autograd graph uses has its accumulation on that graph's stream.  The
-// engine would make that stream wait for the captured one, which ends the capture and then the process;
-// called in a backward pass, before anything is enqueued.
+// A leaf that an earlier, living autograd graph uses has its accumulation on that graph's stream, and so has
+// every node of that graph.  The engine would make that stream wait for the captured one, which ends the
+// capture and then the process; called in a backward pass, before anything is enqueued.  Looks at all that
+// this pass still has to run behind the current node: a leaf may stand behind views and copies of it.
 void check_capture(const char* what) {
   if (!capturing(c10::hip::getCurrentHIPStream().stream())) return;
-  const auto node = torch::autograd::get_current_node();
-  if (!node) return;
-  for (size_t i = 0; i < node->num_outputs(); ++i) {
-    const auto& next = node->next_edge(i).function;
-    if (!node->task_should_compute_output(i) || !dynamic_cast<torch::autograd::AccumulateGrad*>(next.get())) continue;
-    const auto s = next->stream();
-    if (!s) continue;
-    const c10::Stream h(c10::Stream::UNSAFE, c10::Device(c10::DeviceType::HIP, s->device_index()), s->id());
-    TORCH_CHECK(capturing(c10::hip::HIPStream(c10::hip::HIPStream::UNCHECKED, h).stream()), "dgprf: ", what,
-                ": this backward pass is being captured while an autograd graph from before the capture holds one "
-                "of its leaves; delete that graph's results first");
+  const auto current = torch::autograd::get_current_node();
+  if (!current) return;
+  std::vector<torch::autograd::Node*> open{current.get()};
+  std::unordered_set<torch::autograd::Node*> seen{current.get()};
+  while (!open.empty()) {
+    torch::autograd::Node* const node = open.back();
+    open.pop_back();
+    for (size_t i = 0; i < node->num_outputs(); ++i) {
+      torch::autograd::Node* const next = node->next_edge(i).function.get();
+      if (!next || !node->task_should_compute_output(i) || !seen.insert(next).second) continue;
+      if (const auto s = next->stream()) {
+        const c10::Stream h(c10::Stream::UNSAFE, c10::Device(c10::DeviceType::HIP, s->device_index()), s->id());
+        TORCH_CHECK(capturing(c10::hip::HIPStream(c10::hip::HIPStream::UNCHECKED, h).stream()), "dgprf: ", what,
+                    ": this backward pass is being captured while an autograd graph from before the capture holds one "
+                    "of its leaves; delete that graph's results first");
+      }
+      open.push_back(next);
+    }
   }
 }
 

@@ -426,6 +426,35 @@ def test_capture_beside_an_eager_graph():
         del y
 
 
+def test_capture_beside_an_eager_graph_of_a_viewed_leaf():
+    """The same refusal where a leaf stands behind a view, a copy or other operations, whose nodes are new
+    while the leaf's is the living graph's."""
+    x, w = torch.ones(2, 3, 8, device=DEV, requires_grad=True), torch.ones(8, 8, device=DEV, requires_grad=True)
+    b = torch.ones(16, device=DEV, requires_grad=True)
+    dy = torch.ones(2, 3, 8, device=DEV)
+    x0, w0 = x.detach(), w.detach()
+    for op, of in ((lambda: dgprf.linear(x, w0), x), (lambda: dgprf.linear(x0, w.t()), w),
+                   (lambda: dgprf.linear(x0, w0, b[::2]), b), (lambda: dgprf.dropout(2 * x, 0.0), x),
+                   (lambda: dgprf.linear(x0, w0, residual=x * x), x),
+                   (lambda: dgprf.linear(dgprf.dropout(x, 0.0), w0), x)):
+        held = op()
+        with pytest.raises(RuntimeError, match="being captured"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                y = op()
+                torch.autograd.grad(y, of, dy)
+        want = torch.autograd.grad(held, of, dy)[0]
+        del held, y
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = op()
+            got, = torch.autograd.grad(y, of, dy)
+        for _ in range(2):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+        del y
+
+
 def test_two_graphs_and_streams():
     """Two captured calls do not share scratch, and a call on another stream is ordered there."""
     g = _gen(8)
