@@ -258,6 +258,14 @@ void dense_like(const Tensor& t, const Tensor& x, const char* what) {
   TORCH_CHECK_VALUE(t.device() == x.device(), "dgprf: ", what, " is on ", t.device(), ", x is on ", x.device());
 }
 bool given(const OptT& t) { return t.has_value() && t->defined(); }
+// A forward-mode tangent would be left out silently (a dual tensor need not ask for a gradient): an error.
+void no_tangent(const Tensor& t, const char* what) {
+  TORCH_CHECK(!t.defined() || !t._fw_grad(/*level=*/0).defined(), "dgprf: ", what,
+              " has no forward-mode derivative; use torch.autograd.grad");
+}
+void no_tangent(const OptT& t, const char* what) {
+  if (t.has_value()) no_tangent(*t, what);
+}
 
 // [..., n] as a matrix that the kernels can read: unit stride within a row, rows apart by 0 or by n and
 // more.  A view where the strides allow one.
@@ -398,6 +406,7 @@ struct LinearFunction : public torch::autograd::Function<LinearFunction> {
     const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
     const bool want_b = bias && ctx->needs_input_grad(2), want_r = res && ctx->needs_input_grad(bias ? 3 : 2);
     const c10::DeviceGuard guard(x.device());
+    no_tangent(grads[0], "linear's gradient");
     check_capture("linear");
     Tensor dx, dw, db;
     if (want_x || want_w || want_b) {
@@ -448,6 +457,7 @@ struct DropoutFunction : public torch::autograd::Function<DropoutFunction> {
     const Tensor step = ctx->get_saved_variables()[0];
     const auto args = ctx->saved_data["args"].toIntVector();
     const c10::DeviceGuard guard(grads[0].device());
+    no_tangent(grads[0], "dropout's gradient");
     check_capture("dropout");
     Tensor dx;
     if (ctx->needs_input_grad(0)) {
@@ -466,6 +476,10 @@ constexpr const char* kNoCpu = ": the dense operators need a HIP device (there i
 Tensor linear(const Tensor& x, const Tensor& weight, const OptT& bias, int64_t act, const OptT& residual,
               int64_t thr, int64_t seed, int64_t sub, const OptT& step) {
   dense_type(x, "x");
+  no_tangent(x, "linear");
+  no_tangent(weight, "linear");
+  no_tangent(bias, "linear");
+  no_tangent(residual, "linear");
   TORCH_CHECK(x.is_cuda(), "dgprf: x is on ", x.device(), kNoCpu);
   dense_like(weight, x, "weight");
   TORCH_CHECK_VALUE(x.dim() >= 1 && weight.dim() == 2 && x.size(-1) == weight.size(0),
@@ -498,6 +512,8 @@ Tensor linear(const Tensor& x, const Tensor& weight, const OptT& bias, int64_t a
 
 Tensor dropout(const Tensor& x, const OptT& residual, int64_t thr, int64_t seed, int64_t sub, const OptT& step) {
   dense_type(x, "x");
+  no_tangent(x, "dropout");
+  no_tangent(residual, "dropout");
   TORCH_CHECK(x.is_cuda(), "dgprf: x is on ", x.device(), kNoCpu);
   TORCH_CHECK_VALUE(x.dim() >= 1, "dgprf: x must have at least one dimension");
   const int64_t n = x.size(-1);

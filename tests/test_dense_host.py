@@ -120,6 +120,21 @@ def test_python_refusals():
     assert [dgprf.dense.drop_threshold(p) for p in (0, 0.1, 0.5, 1)] == [0, 6554, 32768, 65536]
 
 
+@pytest.mark.parametrize("which", range(4))
+def test_forward_mode_refused(which):
+    """A dual tensor need not ask for a gradient; its tangent is not dropped silently."""
+    import torch.autograd.forward_ad as fw
+    args = [torch.ones(4, 8), torch.ones(8, 16), torch.ones(16), torch.ones(4, 16)]
+    with fw.dual_level():
+        args[which] = fw.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            dgprf.linear(*args[:3], residual=args[3])
+        if which in (0, 3):
+            pair = [fw.make_dual(torch.ones(4, 8), torch.ones(4, 8)), torch.ones(4, 8)]
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                dgprf.dropout(pair[which > 0], 0.5, residual=pair[which == 0])
+
+
 def test_layer_refusals():
     from layers import DenseLayer, DropoutLayer
     for bad in (lambda: DenseLayer(4, 8, activation="tanh"), lambda: DenseLayer(4, 8, dropout=2.0),

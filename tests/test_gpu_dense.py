@@ -552,6 +552,25 @@ def test_refusals():
         torch.autograd.grad(y.sum(), wg)
 
 
+def test_forward_mode_refused():
+    """A tangent of any argument, and of the gradient that a backward pass gets, is an error."""
+    import torch.autograd.forward_ad as fw
+    args = [torch.ones(s, device=DEV) for s in ((4, 8), (8, 16), (16,), (4, 16))]
+    for which in range(4):
+        for asks in (False, True):  # another argument asks for a gradient, or none does
+            with fw.dual_level():
+                a = [v.clone().requires_grad_(asks) for v in args]
+                a[which] = fw.make_dual(args[which], torch.ones_like(args[which]))
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    dgprf.linear(*a[:3], residual=a[3])
+    for op, leaf in ((lambda v: dgprf.linear(v, args[1]), (4, 8)), (lambda v: dgprf.dropout(v, 0.5), (4, 16))):
+        v = torch.ones(leaf, device=DEV, requires_grad=True)
+        y = op(v)
+        with fw.dual_level():
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(y, v, fw.make_dual(args[3], torch.ones_like(y)))
+
+
 def test_offsets_past_32_bits():
     """65,600 rows of 32,768 elements: the last rows of a result, and gradients over all of them."""
     m, k, n, t = 65600, 16, 32768, torch.bfloat16
