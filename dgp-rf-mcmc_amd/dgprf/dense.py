@@ -7,8 +7,11 @@ Both are differentiable (torch.autograd); the backward pass makes the mask again
 counters.  They run on torch's current stream of the tensors' device and can be captured by
 torch.cuda.graph.  include/dgprf.h (dgprf_linear_t) has the definition of the mask.
 """
+import torch
+
 from . import _native as N
 from . import engine as E
+
 
 def drop_threshold(p):
     """The share of 65536 that dropout of probability p drops (p is rounded to a multiple of it)."""
@@ -24,6 +27,13 @@ def _stream_of(thr, seed, sub, step):
     itself: step is added to sub, and no other call's masks may come up."""
     if thr == 0:
         return 0, 0
+    if sub is None and thr < 65536:  # (p = 1 drops everything whatever the number)
+        # A forward pass that a backward pass runs again (activation checkpointing) would draw another
+        # mask than the result that it stands for was made with.
+        if torch._C._current_graph_task_id() != -1:
+            raise RuntimeError(
+                "dgprf: dropout inside a backward pass (activation checkpointing runs the forward pass again "
+                "there) needs sub given: the generator's next number would give another mask than before")
     if seed is None:
         seed = E._RNG.seed
     if sub is None:
@@ -38,7 +48,9 @@ def linear(x, weight, bias=None, activation="none", residual=None, dropout=0.0, 
     x [..., k], weight [k, n] (GPLayer's layout), bias [n], residual of y's shape [..., n]; one type
     of float32, float16 and bfloat16 for all.  activation: none, relu, gelu, gelu_tanh or silu.
     dropout: the probability p of an element's being dropped, rounded to a multiple of 1 / 65536.
-    seed / sub: key and number of the mask (default: the global generator, its next subsequence);
+    seed / sub: key and number of the mask (default: the global generator, its next subsequence; a call
+    that activation checkpointing runs again in the backward pass needs sub given, so that it makes the
+    same mask, and raises RuntimeError without);
     step: an int64 device tensor added to sub when the kernels run, for a captured call — advance it
     after the call's backward pass, and keep given subs of different calls more than the number of
     steps apart.  The gradient of the gradient is not available.

@@ -135,6 +135,42 @@ def test_forward_mode_refused(which):
                 dgprf.dropout(pair[which > 0], 0.5, residual=pair[which == 0])
 
 
+class _StandIn:
+    """dgprf.dropout's operator on the CPU: the mask of (seed, sub) by torch's generator."""
+
+    @staticmethod
+    def dropout(x, residual, thr, seed, sub, step):
+        g = torch.Generator()
+        g.manual_seed((seed * 31 + sub) % 2 ** 62)
+        return x * (torch.rand(x.shape, generator=g) >= thr / 65536)
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_recomputed_masks(monkeypatch, reentrant):
+    """A forward pass that activation checkpointing runs again draws no other mask: default numbers are
+    refused there, given ones make the same mask."""
+    from torch.utils.checkpoint import checkpoint
+    monkeypatch.setattr(dgprf.dense.E, "ops", lambda: _StandIn)
+    x = torch.linspace(-1, 1, 64).requires_grad_()
+
+    def run(**kw):
+        y = checkpoint(lambda v: dgprf.dropout(v, 0.5, **kw).square(), x, use_reentrant=reentrant)
+        x.grad = None
+        y.sum().backward()
+        return y.detach()
+
+    for kw in ({}, dict(seed=3), dict(step=torch.zeros(1, dtype=torch.int64))):
+        with pytest.raises(RuntimeError, match="needs sub"):
+            run(**kw)
+    y = run(seed=3, sub=4)
+    assert torch.equal(x.grad != 0, y != 0) and 0 < int((y != 0).sum()) < 64
+    run(sub=4)
+    # nothing to draw: no mask, and all of it
+    monkeypatch.setattr(_StandIn, "dropout", staticmethod(lambda x, r, thr, *a: x * (thr == 0)))
+    for p in (0.0, 1.0):
+        checkpoint(lambda v: dgprf.dropout(v, p).square(), x, use_reentrant=reentrant).sum().backward()
+
+
 def test_layer_refusals():
     from layers import DenseLayer, DropoutLayer
     for bad in (lambda: DenseLayer(4, 8, activation="tanh"), lambda: DenseLayer(4, 8, dropout=2.0),

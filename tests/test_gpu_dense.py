@@ -571,6 +571,31 @@ def test_forward_mode_refused():
                 torch.autograd.grad(y, v, fw.make_dual(args[3], torch.ones_like(y)))
 
 
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_activation_checkpointing(reentrant):
+    """A recomputed forward pass makes the masks that are given, and the same gradients; it does not draw
+    the generator's next ones."""
+    from torch.utils.checkpoint import checkpoint
+    g = _gen(12)
+    x, w = normal(g, 40, 24).to(DEV).requires_grad_(), normal(g, 24, 56, scale=0.2).to(DEV).requires_grad_()
+    dy = normal(g, 40, 56).to(DEV)
+
+    def run(wrap, sub):
+        # (a dropout at the end would not be run again: it saves nothing)
+        f = lambda v: dgprf.linear(dgprf.dropout(v, 0.4, sub=sub[0]), w, activation="gelu", dropout=0.3, sub=sub[1])  # noqa: E731
+        y = checkpoint(f, x, use_reentrant=reentrant) if wrap else f(x)
+        x.grad = w.grad = None
+        y.backward(dy)
+        return y.detach(), x.grad, w.grad
+
+    assert all(torch.equal(u, v) for u, v in zip(run(True, (5, 6)), run(False, (5, 6))))
+    for sub in ((5, None), (None, 6), (None, None)):
+        run(False, sub)
+        with pytest.raises(RuntimeError, match="needs sub"):
+            run(True, sub)
+    torch.cuda.synchronize()
+
+
 def test_offsets_past_32_bits():
     """65,600 rows of 32,768 elements: the last rows of a result, and gradients over all of them."""
     m, k, n, t = 65600, 16, 32768, torch.bfloat16
