@@ -21,7 +21,15 @@ def drop_threshold(p):
     return int(p * 65536 + 0.5)
 
 
-def _stream_of(thr, seed, sub, step):
+def _captured(x):
+    """Whether calls on x are being captured into a graph."""
+    if not (torch.is_tensor(x) and x.is_cuda) or torch._C._cuda_getCurrentRawStream(x.get_device()) == 0:
+        return False  # (the null stream cannot be captured, and must not be asked while another is)
+    with torch.cuda.device(x.device):
+        return torch.cuda.is_current_stream_capturing()
+
+
+def _stream_of(x, thr, seed, sub, step):
     """(seed, sub) of this call's mask: as given, or the global generator's key and its next
     subsequence (dgprf.set_seed makes a run's masks repeat).  With a step, the call has 2^32 of them to
     itself: step is added to sub, and no other call's masks may come up."""
@@ -34,6 +42,10 @@ def _stream_of(thr, seed, sub, step):
             raise RuntimeError(
                 "dgprf: dropout inside a backward pass (activation checkpointing runs the forward pass again "
                 "there) needs sub given: the generator's next number would give another mask than before")
+        if step is None and _captured(x):
+            raise RuntimeError(
+                "dgprf: dropout captured into a graph needs step (a device counter), or sub given for one mask "
+                "in every replay: the generator's number would be drawn once, for all replays")
     if seed is None:
         seed = E._RNG.seed
     if sub is None:
@@ -53,13 +65,14 @@ def linear(x, weight, bias=None, activation="none", residual=None, dropout=0.0, 
     same mask, and raises RuntimeError without);
     step: an int64 device tensor added to sub when the kernels run, for a captured call — advance it
     after the call's backward pass, and keep given subs of different calls more than the number of
-    steps apart.  The gradient of the gradient is not available.
+    steps apart.  A captured call with neither sub nor step raises RuntimeError (its mask would be one for
+    all replays); with sub alone it repeats the mask of sub.  The gradient of the gradient is not available.
     """
     act = N.ACTS.get(activation)
     if act is None:
         raise ValueError(f"activation must be one of {', '.join(N.ACTS)}, got {activation!r}")
     thr = drop_threshold(dropout) if dropout else 0
-    seed, sub = _stream_of(thr, seed, sub, step)
+    seed, sub = _stream_of(x, thr, seed, sub, step)
     return E.ops().linear(x, weight, bias, act, residual, thr, seed, sub, step)
 
 
@@ -67,5 +80,5 @@ def dropout(x, p, residual=None, seed=None, sub=None, step=None):
     """y = residual + s m x for x [..., n]: the mask of `linear`'s result of the same rows, (seed, sub)
     and n.  p = 1 drops everything.  Arguments as in `linear`."""
     thr = drop_threshold(p)
-    seed, sub = _stream_of(thr, seed, sub, step)
+    seed, sub = _stream_of(x, thr, seed, sub, step)
     return E.ops().dropout(x, residual, thr, seed, sub, step)

@@ -171,6 +171,21 @@ def test_recomputed_masks(monkeypatch, reentrant):
         checkpoint(lambda v: dgprf.dropout(v, p).square(), x, use_reentrant=reentrant).sum().backward()
 
 
+def test_captured_masks(monkeypatch):
+    """A captured call does not draw a number that all its replays would share."""
+    seen = []
+    monkeypatch.setattr(_StandIn, "dropout", staticmethod(lambda *a: seen.append(a)))
+    monkeypatch.setattr(dgprf.dense.E, "ops", lambda: _StandIn)
+    monkeypatch.setattr(dgprf.dense, "_captured", lambda x: True, raising=False)
+    x, step = torch.ones(8), torch.zeros(1, dtype=torch.int64)
+    for kw in ({}, dict(seed=3)):
+        with pytest.raises(RuntimeError, match="needs step"):
+            dgprf.dropout(x, 0.5, **kw)
+    for p, kw in ((0.5, dict(step=step)), (0.5, dict(sub=2)), (0.5, dict(sub=2, step=step)), (0.0, {}), (1.0, {})):
+        dgprf.dropout(x, p, **kw)
+    assert len(seen) == 5
+
+
 def test_layer_refusals():
     from layers import DenseLayer, DropoutLayer
     for bad in (lambda: DenseLayer(4, 8, activation="tanh"), lambda: DenseLayer(4, 8, dropout=2.0),

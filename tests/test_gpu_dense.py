@@ -571,6 +571,33 @@ def test_forward_mode_refused():
                 torch.autograd.grad(y, v, fw.make_dual(args[3], torch.ones_like(y)))
 
 
+def test_captured_masks_are_drawn_on_each_replay():
+    """Captured with neither sub nor step, a call is refused; with a step every replay has a mask of its
+    own, with sub alone all have the mask of sub."""
+    from layers import DenseLayer
+    x, w = torch.ones(16, 64, device=DEV), torch.eye(64, device=DEV)
+    step = torch.zeros(1, dtype=torch.int64, device=DEV)
+    layer = DenseLayer(64, 64, dropout=0.5)
+    layer.set_training(True)
+    for op in (lambda: dgprf.dropout(x, 0.5), lambda: dgprf.linear(x, w, dropout=0.5, seed=4), lambda: layer(x)):
+        op()
+        with pytest.raises(RuntimeError, match="needs step"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                x + 1
+                op()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, z, u = dgprf.dropout(x, 0.5, step=step), dgprf.dropout(x, 0.5, sub=9), dgprf.dropout(x, 1.0)
+        step += 1
+    masks = []
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        masks.append(y.clone())
+        assert torch.equal(z, dgprf.dropout(x, 0.5, sub=9)) and not bool(u.any())
+    assert not any(torch.equal(masks[i], masks[j]) for i, j in ((0, 1), (0, 2), (1, 2)))
+
+
 @pytest.mark.parametrize("reentrant", [False, True])
 def test_activation_checkpointing(reentrant):
     """A recomputed forward pass makes the masks that are given, and the same gradients; it does not draw
