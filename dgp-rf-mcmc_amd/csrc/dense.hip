@@ -250,9 +250,10 @@ __global__ __launch_bounds__(1024) void k_strip(const T* __restrict__ x, const T
 }
 
 // ---------------------------------------------------------------- dz and its column sums
-// dz = s m dy a'(z) (rounded to the tensors' type, as the matrix instructions take it; its sums for
+// dz / s = m dy a'(z) (rounded to the tensors' type, as the matrix instructions take it; its sums for
 // db are of the unrounded values), one thread for eight columns and `rows_part` rows; dz is null
-// where it would equal dy.  Workgroups behind those pack the products' other operands, which saves odd
+// where it would equal dy.  s is applied to the products and to db in 32 bits, because in fp16 s dy
+// overflows where their results need not (p = 0.75: from dy = 16376 on).  Workgroups behind those pack the products' other operands, which saves odd
 // sizes a launch (dx of 700 x 700 over 3500 in bf16: 28.9 us, 34.7 with two).
 struct DzDev {
   const void* dy;
@@ -331,10 +332,10 @@ __global__ __launch_bounds__(256) void k_dz(const DzDev d, const PackDev a, cons
   }
 }
 
-// db[c] = sum of the parts: 32 columns of a workgroup, 32 threads each, in a fixed order
+// db[c] = s times the sum of the parts: 32 columns of a workgroup, 32 threads each, in a fixed order
 template <class T>
 __global__ __launch_bounds__(1024) void k_db(const float* __restrict__ part, int64_t ldp, int parts, int N,
-                                             T* __restrict__ db) {
+                                             float s_drop, T* __restrict__ db) {
   __shared__ float sums[32][33];
   const int cl = threadIdx.x & 31, r = threadIdx.x >> 5, c = blockIdx.x * 32 + cl;
   float s = 0.f;
@@ -348,7 +349,7 @@ __global__ __launch_bounds__(1024) void k_db(const float* __restrict__ part, int
     if (r < h) sums[r][cl] += sums[r + h][cl];
     __syncthreads();
   }
-  if (r == 0 && c < N) db[c] = (T)sums[0][cl];
+  if (r == 0 && c < N) db[c] = (T)(s_drop * sums[0][cl]);
 }
 
 // ---------------------------------------------------------------- dropout
@@ -557,12 +558,14 @@ hipError_t product(int dtype, int layout, const void* A, int64_t lda, const void
   return err;
 }
 
-EpiDev epi_plain(void* y, int64_t n) {
+// y = s times the product
+EpiDev epi_plain(void* y, int64_t n, float s) {
   EpiDev e{};
   e.y = y;
   e.ldy = n;
   e.n = (int)n;
   e.groups = (int)cdiv(n, 8);
+  e.drop.scale = s;
   return e;
 }
 
@@ -584,7 +587,7 @@ int check_dims(int32_t dtype, int32_t act, int64_t m, int64_t k, int64_t n, int6
 hipError_t forward(const dgprf_linear_t& a, Scratch& sc, hipStream_t st, bool run) {
   const int es = elem_size(a.dtype);
   const int64_t m = a.m, k = a.k, n = a.n;
-  EpiDev e = epi_plain(a.y, n);
+  EpiDev e = epi_plain(a.y, n, 1.f);
   e.bias = a.bias;
   e.res = a.res;
   e.aux = a.act != DGPRF_ACT_NONE ? a.aux : nullptr;
@@ -627,7 +630,8 @@ hipError_t backward(const dgprf_linear_grad_t& a, Scratch& sc, hipStream_t st, b
   const int es = elem_size(a.dtype);
   const int64_t m = a.m, k = a.k, n = a.n;
   hipError_t err = hipSuccess;
-  // dz, unless it is dy and dy can be read in place
+  const DropDev drop = drop_dev(a.drop_thr, a.seed, a.sub, a.step);
+  // dz / s, unless it is dy and dy can be read in place
   const bool products = a.dx || a.dw;
   // (rows that share memory are copied apart: their product's K range has no end to check against)
   const bool same = a.act == DGPRF_ACT_NONE && a.drop_thr == 0 && a.lddy >= n && in_place(a.dy, a.lddy, n, es);
@@ -652,7 +656,8 @@ hipError_t backward(const dgprf_linear_grad_t& a, Scratch& sc, hipStream_t st, b
     d.N = (int)n;
     d.groups = (int)cdiv(n, 8);
     d.act = a.act;
-    d.drop = drop_dev(a.drop_thr, a.seed, a.sub, a.step);
+    d.drop = drop;
+    d.drop.scale = 1.f;
     d.strips = (int)cdiv(d.groups, 64);
     // workgroups enough to fill the chip, down to a row for each wave
     const int64_t want = std::max<int64_t>(1, std::min<int64_t>(cdiv(1024, d.strips), cdiv(m, 4)));
@@ -667,7 +672,7 @@ hipError_t backward(const dgprf_linear_grad_t& a, Scratch& sc, hipStream_t st, b
         hipError_t er = hipGetLastError();
         if (er == hipSuccess && a.db) {
           hipLaunchKernelGGL((k_db<T>), dim3((unsigned)cdiv(n, 32)), dim3(1024), 0, st, d.part, d.ldz, d.parts,
-                             (int)n, (T*)a.db);
+                             (int)n, drop.scale, (T*)a.db);
           er = hipGetLastError();
         }
         return er;
@@ -677,12 +682,12 @@ hipError_t backward(const dgprf_linear_grad_t& a, Scratch& sc, hipStream_t st, b
   } else if (run && (err = pack(a.dtype, pw, px, st)) != hipSuccess) {
     return err;
   }
-  if (a.dx) {  // [m][k] = dz [m][n] (W [k][n])^T
-    err = product(a.dtype, LAYOUT_NT, dz, lddz, w, ldw, m, k, 0, 0, na, nb, epi_plain(a.dx, k), sc, st, run);
+  if (a.dx) {  // [m][k] = s (dz / s) [m][n] (W [k][n])^T
+    err = product(a.dtype, LAYOUT_NT, dz, lddz, w, ldw, m, k, 0, 0, na, nb, epi_plain(a.dx, k, drop.scale), sc, st, run);
     if (err != hipSuccess) return err;
   }
-  if (a.dw)  // [k][n] = (x [m][k])^T dz [m][n]
-    err = product(a.dtype, LAYOUT_TN, x, ldx, dz, lddz, k, n, ka, na, m, m, epi_plain(a.dw, n), sc, st, run);
+  if (a.dw)  // [k][n] = s (x [m][k])^T (dz / s) [m][n]
+    err = product(a.dtype, LAYOUT_TN, x, ldx, dz, lddz, k, n, ka, na, m, m, epi_plain(a.dw, n, drop.scale), sc, st, run);
   return err;
 }
 

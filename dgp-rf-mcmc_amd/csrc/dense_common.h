@@ -137,7 +137,7 @@ __device__ __forceinline__ float saved_of(float z) {
 // number, so the mask does not depend on how a kernel is tiled and backward makes it again.
 struct DropDev {
   uint32_t thr;  // an element is kept when its 16 bits >= thr; 0: no dropout, 65536: drops all
-  float scale;   // 65536 / (65536 - thr); 0 when everything is dropped
+  float scale;   // 65536 / (65536 - thr); 0 when everything is dropped (with thr = 0: of all elements)
   uint32_t k0, k1;
   uint64_t sub;
   const int64_t* step;  // device counter added to sub, or null
@@ -298,8 +298,12 @@ __device__ __forceinline__ F8 value_of(const EpiDev& e, int64_t row, int col, ui
       v.hi[c] = act_of<T, ACT>(v.hi[c]);
     }
   }
-  if (e.drop.thr)
+  if (e.drop.thr) {
     v = drop8(v, drop_words(e.drop, sub, (uint64_t)row * (uint32_t)e.groups + (uint32_t)(col >> 3)), e.drop);
+  } else if (ACT == DGPRF_ACT_NONE && e.drop.scale != 1.f) {  // the products of a backward pass
+    v.lo *= e.drop.scale;
+    v.hi *= e.drop.scale;
+  }
   return v;
 }
 

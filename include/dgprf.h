@@ -421,7 +421,7 @@ int dgprf_mass_estimate(const dgprf_plan_t *plan, const float *mean, const float
  *
  * All tensors of a call have one element type (DGPRF_F32 / F16 / BF16) and unit stride within a row.
  * Sums, bias, activation, mask and residual are in 32 bits; a value is rounded once, where it is
- * stored.  16-bit backward passes round dz to the type before its two products.
+ * stored.  16-bit backward passes round dz / s to the type before its two products.
  * Sizes: k, n and the row strides up to 2^20, m up to 2^31 - 512, results up to 2^38 elements; m = 0 is
  * allowed. */
 #define DGPRF_F32 0

@@ -174,6 +174,26 @@ def test_dropout(shape, p, tname):
     assert torch.equal(dgprf.dropout(x.to(DEV), p, seed=seed, sub=sub).cpu(), drop(x).to(t))
 
 
+@pytest.mark.parametrize("act", ["none", "silu"])
+@pytest.mark.parametrize("size", [(40, 24, 56), (400, 72, 520)], ids=str)
+def test_gradients_where_scaled_ones_overflow(size, act):
+    """fp16: s dy is above the type's largest value, dx and dW are not."""
+    t, g = torch.float16, _gen(13)
+    m, k, n = size
+    for p, top in ((0.75, 30000), (65535 / 65536, 1)):
+        x, w = normal(g, m, k, t=t, scale=2.0 ** -9), normal(g, k, n, t=t, scale=2.0 ** -10)
+        dy = (torch.randint(0, 2, (m, n), generator=g) * 2 - 1).to(t) * top
+        thr = int(p * 65536 + 0.5)
+        ref = Linear(x, w, None, act, None, thr, 1, 2, dy)
+        assert float(ref.dx.abs().max()) < 60000 and float(ref.dw.abs().max()) < 60000 < scale_of(thr) * top
+        assert n < 100 or bool(ref.dx.any())
+        _, dx, dw, _, _ = run(x, w, None, act, None, p, 1, 2, dy)
+        # dz / s is stored, so its smallest step counts s times
+        more = scale_of(thr) * torch.finfo(t).smallest_normal * torch.finfo(t).eps
+        check(dx, ref.dx, ref.dx_tol + more * w.double().abs().sum(1), "dx")
+        check(dw, ref.dw, ref.dw_tol + more * x.double().abs().sum(0)[:, None], "dw")
+
+
 def test_linear_takes_dropouts_mask():
     """The mask depends on (seed, sub, row, column, n) alone: every path of linear has the one of dropout."""
     for m, n in ((1, 40), (7, 136), (20, 264), (150, 100), (513, 130), (4096, 2560)):
