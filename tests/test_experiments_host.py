@@ -77,6 +77,35 @@ def test_adam_matches_keras_rule():
     assert opt.iterations == 4
 
 
+@pytest.mark.parametrize("t", [torch.float16, torch.bfloat16])
+def test_adam_of_16_bit_variables(t):
+    """The rule in float64 on the same gradients, rounded to the type where it is stored: a small gradient
+    whose square underflows, steps far below the variable's last place, and a value assigned in between.
+    Off by half a step of the type, and 32-bit rounding: 2^-24 of the value and some 2^-17 of the learning
+    rate (sums of m and v, their quotient) for each step."""
+    from experiments.optimizers import Adam
+    rng = np.random.default_rng(4)
+    var = torch.tensor(np.append(0.05 * rng.standard_normal(200), [1.0, -1.0, 3.0]), dtype=t).requires_grad_()
+    want, m, v = var.detach().double().numpy().copy(), 0.0, 0.0
+    opt, lr, steps, half = Adam(learning_rate=1e-3), 1e-3, 30, torch.finfo(t).eps / 2
+    first = want.copy()
+    for i in range(1, steps + 1):
+        # same signs in the last three, so that they move one way
+        g = torch.tensor(1e-3 * np.append(rng.standard_normal(200), [1.0, 0.5, -2.0]), dtype=t)
+        if i == 20:
+            with torch.no_grad():
+                var[7] = 0.5
+            want[7] = 0.5
+        opt.apply_gradients([(g, var)])
+        want, m, v = O.adam_update(want, g.double().numpy(), m, v, i, lr=lr)
+        err = i * (2.0 ** -24 * np.abs(want) + 2.0 ** -17 * lr)
+        tol = half * (np.abs(want) + err) + err + float(torch.finfo(t).smallest_normal * torch.finfo(t).eps)
+        off = np.abs(var.detach().double().numpy() - want)
+        assert (off <= tol).all(), (i, off.max(), (off - tol).argmax())
+    assert np.abs(want - first)[200:].min() > 0.02  # the last three did move
+    assert opt.get_slot(var, "v").dtype == torch.float32
+
+
 # ----------------------------------------------------------------------------- datasets
 def _write_csv(tmp_path, name, N, D, seed=0):
     rng = np.random.default_rng(seed)
