@@ -35,6 +35,8 @@ class DenseLayer(Module):
             raise ValueError(f"activation must be one of {', '.join(N.ACTS)}, got {activation!r}")
         if not 0. <= dropout <= 1.:
             raise ValueError(f"dropout probability must be in [0, 1], got {dropout}")
+        if dtype not in (torch.float32, torch.float16, torch.bfloat16):
+            raise TypeError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
         self.in_feature, self.out_feature = int(in_feature), int(out_feature)
         self.activation, self.dropout, self.training = activation, float(dropout), False
         w = E.normal((self.in_feature, self.out_feature), N.RNG_W) * self.in_feature ** -0.5

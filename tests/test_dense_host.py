@@ -194,6 +194,14 @@ def test_layer_refusals():
             bad()
 
 
+@pytest.mark.parametrize("dtype", [torch.float64, torch.int32, torch.complex64, "float32", None])
+def test_layer_types_refused(dtype):
+    """When the layer is made, not at its first call."""
+    from layers import DenseLayer
+    with pytest.raises(TypeError, match="dtype"):
+        DenseLayer(4, 8, dtype=dtype)
+
+
 @pytest.mark.skipif(torch.cuda.is_available(), reason="checks the no-GPU refusal")
 def test_layer_needs_a_device():
     from layers import DenseLayer
