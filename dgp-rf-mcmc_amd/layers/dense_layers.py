@@ -13,13 +13,14 @@ from dgprf.dense import dropout, linear
 from dgprf.module import Module
 
 
-def _input(X, n, dtype):
-    """X [..., n] on the device in the layer's type (a tensor that is, is taken as it is)."""
+def _input(X, W):
+    """X [..., in_feature] on the device of W (not the current one) in its type; a tensor that is, is taken
+    as it is."""
     if not torch.is_tensor(X):
         X = torch.as_tensor(X)
-    if X.dim() < 1 or X.shape[-1] != n:
-        raise ValueError(f"X must be [..., {n}], got {tuple(X.shape)}")
-    return X.to(device=E.device(), dtype=dtype)
+    if X.dim() < 1 or X.shape[-1] != W.shape[0]:
+        raise ValueError(f"X must be [..., {W.shape[0]}], got {tuple(X.shape)}")
+    return X.to(device=W.device, dtype=W.dtype)
 
 
 class DenseLayer(Module):
@@ -49,7 +50,7 @@ class DenseLayer(Module):
 
     def __call__(self, X, residual=None, seed=None, sub=None, step=None):
         """X [..., in_feature] -> [..., out_feature]; seed, sub, step: the mask's, as in dgprf.linear."""
-        X = _input(X, self.in_feature, self.W.dtype)
+        X = _input(X, self.W)
         return linear(X, self.W, self.b, self.activation, residual,
                       self.dropout if self.training else 0., seed, sub, step)
 

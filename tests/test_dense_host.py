@@ -202,6 +202,21 @@ def test_layer_types_refused(dtype):
         DenseLayer(4, 8, dtype=dtype)
 
 
+def test_layer_takes_its_own_device(monkeypatch):
+    """A layer's input goes to where its weights are, whichever device is current."""
+    from layers import DenseLayer, dense_layers
+    layer, seen = DenseLayer.__new__(DenseLayer), []
+    layer.in_feature, layer.out_feature, layer.activation, layer.dropout, layer.training = 4, 8, "none", 0.0, False
+    layer.W, layer.b = torch.zeros(4, 8, dtype=torch.float16), None
+    monkeypatch.setattr(dense_layers.E, "device", lambda: torch.device("meta"))
+    monkeypatch.setattr(dense_layers, "linear", lambda x, *a: seen.append(x))
+    layer(torch.zeros(3, 4))
+    layer([[1.0, 2.0, 3.0, 4.0]])
+    assert all(x.device == layer.W.device and x.dtype == torch.float16 for x in seen) and len(seen) == 2
+    with pytest.raises(ValueError, match="X must be"):
+        layer(torch.zeros(3, 5))
+
+
 @pytest.mark.skipif(torch.cuda.is_available(), reason="checks the no-GPU refusal")
 def test_layer_needs_a_device():
     from layers import DenseLayer
