@@ -39,8 +39,8 @@ def run(x, w, b=None, act="none", r=None, p=0.0, seed=0, sub=0, dy=None, **kw):
     return (y, *(None if v is None else next(got) for v in leaf))
 
 
-# rows of the streaming kernel (1 .. 8), of the 32-row tile, of 128- and 256-wide tiles; K and N below, at
-# and above a 16-byte piece, a fragment, a stage and a tile; one and many parts of K
+# one row, two, rows of the 32-row tile and of larger ones; K and N below, at and above a 16-byte piece, a
+# fragment, a stage and a tile; one and many parts of K
 SIZES = [(1, 1, 1), (1, 64, 64), (1, 2048, 512), (2, 37, 131), (3, 1030, 200), (5, 8, 4096), (8, 1500, 129),
          (9, 1, 7), (9, 64, 128), (17, 515, 33), (32, 4096, 256), (33, 33, 65), (64, 128, 8), (100, 200, 300),
          (128, 64, 128), (129, 1025, 257), (255, 72, 1001), (256, 2048, 256), (700, 9, 700), (1000, 333, 5)]
@@ -95,6 +95,118 @@ def test_large_tiles_in_parts_of_k(size, tname):
     x, w, b, r = draw(m, k), draw(k, n), draw(n), draw(m, n)
     want = 2 * keep_mask(m, n, 32768, 7, 8).to(DEV) * (x.float() @ w.float() + b.float()).clamp(min=0) + r.float()
     assert torch.equal(dgprf.linear(x, w, b, "relu", r, 0.5, 7, 8), want.to(x.dtype))
+
+
+# 16-bit products that, by the rule of sizes, run: x W as 256 x 256 tiles, dz W^T as 128 x 128 in parts;
+# x W as 256 x 128, x^T dz as 128 x 128 in parts; x W as 256 x 128 with two groups; dz W^T as 256 x 256;
+# x^T dz as 256 x 256, and x W as 128 x 128 with two groups; that in parts; x^T dz as 256 x 128 with two groups,
+# in parts; as 256 x 256 in parts; as 128 x 128 in parts; dz W^T as 256 x 128; and some of them with odd sizes
+TILED = [(1500, 776, 8200), (33000, 520, 264), (16400, 72, 136), (8200, 1544, 776), (777, 3000, 4104), (250, 4088, 4104),
+         (16400, 3000, 136), (16400, 4088, 1032), (8200, 776, 264), (33000, 264, 520), (1499, 775, 8199),
+         (32999, 519, 263), (16399, 71, 135), (8199, 1543, 775), (16399, 2999, 135)]
+
+
+@pytest.mark.parametrize("tname", TYPES)
+@pytest.mark.parametrize("size", TILED, ids=str)
+def test_epilogues_of_large_tiles(size, tname):
+    """Bias, relu, mask and residual at once, and all gradients: whole numbers, whose sums are exact."""
+    m, k, n = size
+    t, g = TYPES[tname], torch.Generator(device=DEV)
+    g.manual_seed(m + k + n)
+    draw = lambda *s: torch.randint(-2, 3, s, generator=g, device=DEV).to(t)  # noqa: E731
+    leaf, dy = [v.requires_grad_() for v in (draw(m, k), draw(k, n), draw(n), draw(m, n))], draw(m, n)
+    keep = dgprf.dropout(torch.ones(m, n, device=DEV), 0.5, seed=7, sub=8)  # 0 or 2
+    y = dgprf.linear(*leaf[:3], "relu", leaf[3], 0.5, 7, 8)
+    got = torch.autograd.grad(y, leaf, dy)
+    x, w, b, r = (v.detach().float() for v in leaf)
+    z = x @ w + b
+    dz = dy.float() * keep * (z > 0)
+    want = (keep * z.clamp(min=0) + r, dz @ w.t().contiguous(), x.t().contiguous() @ dz, dz.sum(0), dy)
+    for name, u, v in zip(("y", "dx", "dw", "db", "dr"), (y, *got), want):
+        assert torch.equal(u, v.to(t)), name
+
+
+@pytest.mark.parametrize("tname", TYPES)
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("size", [(1500, 776, 8200), (33000, 519, 264), (16400, 72, 136), (500, 1000, 2056), (250, 4088, 4104)],
+                         ids=str)
+def test_activations_of_large_tiles(size, act, tname):
+    m, k, n = size
+    t, g = TYPES[tname], torch.Generator(device=DEV)
+    g.manual_seed(m + k + n)
+    draw = lambda *s, scale=1.0: (torch.randn(*s, generator=g, device=DEV) * scale).to(t)  # noqa: E731
+    x, w, b, r, dy = draw(m, k), draw(k, n, scale=k ** -0.5), draw(n), draw(m, n), draw(m, n)
+    ref = Linear(x, w, b, act, r, dy=dy)
+    leaf = [v.requires_grad_() for v in (x, w, b)]
+    y = dgprf.linear(*leaf, act, r)
+    dx, dw, db = torch.autograd.grad(y, leaf, dy)
+    for name, u, v, tol in (("y", y, ref.y, ref.y_tol), ("dx", dx, ref.dx, ref.dx_tol), ("dw", dw, ref.dw, ref.dw_tol),
+                            ("db", db, ref.db, ref.db_tol)):
+        check(u, v.cpu(), tol.cpu(), name)
+
+
+@pytest.mark.parametrize("tname", TYPES)
+@pytest.mark.parametrize("act", ["none", "gelu", "silu"])
+@pytest.mark.parametrize("size", [(1, 2049, 300), (1, 5000, 1031), (2, 2052, 1000), (2, 4099, 333), (1, 2048, 1031), (2, 2048, 520)],
+                         ids=str)
+def test_one_and_two_rows(size, act, tname):
+    """Long sums of one row and two, with everything in the epilogue."""
+    m, k, n = size
+    t, g = TYPES[tname], _gen(m + k + n)
+    x, w, b, r = normal(g, m, k, t=t), normal(g, k, n, t=t, scale=k ** -0.5), normal(g, n, t=t), normal(g, m, n, t=t)
+    dy = normal(g, m, n, t=t)
+    ref = Linear(x, w, b, act, r, int(0.3 * 65536 + 0.5), 3, 4, dy)
+    y, dx, dw, db, dr = run(x, w, b, act, r, 0.3, 3, 4, dy)
+    for name, u, v, tol in (("y", y, ref.y, ref.y_tol), ("dx", dx, ref.dx, ref.dx_tol), ("dw", dw, ref.dw, ref.dw_tol),
+                            ("db", db, ref.db, ref.db_tol)):
+        check(u, v, tol, name)
+    assert torch.equal(dr.cpu(), dy)
+
+
+@pytest.mark.parametrize("tname", TYPES)
+@pytest.mark.parametrize("m, k", [(1, 72), (1, 2100), (2, 72), (2, 2100)])
+def test_strides_of_one_and_two_rows(m, k, tname):
+    """Weights, inputs and residuals inside larger tensors, at any offset, and transposed ones: the results
+    of contiguous copies."""
+    t, g, n = TYPES[tname], _gen(m + k), 104
+    base, wide = grid(g, m, k + 24, t=t).to(DEV), grid(g, k + 2, n + 9, t=t).to(DEV)
+    res, row = grid(g, m, n + 9, t=t).to(DEV), grid(g, 1, n, t=t).to(DEV)
+    bias = grid(g, n + 9, t=t).to(DEV)
+    for off in (0, 1, 8):
+        for x, w, r in ((base[:, off:off + k], wide[1:k + 1, off:off + n], res[:, off:off + n]),
+                        (base[:, :k], wide[off % 2:k + off % 2, :n], row.expand(m, n)),
+                        (base[:, :k].t().contiguous().t(), wide[:k, :n].t().contiguous().t(), res[:, off:off + n])):
+            b = bias[off:off + n]
+            y = dgprf.linear(x, w, b, "relu", r, 0.25, 5, 6)
+            c = [v.clone(memory_format=torch.contiguous_format) for v in (x, w, b, r)]
+            assert torch.equal(y, dgprf.linear(*c[:3], "relu", c[3], 0.25, 5, 6))
+            keep = 4 / 3 * keep_mask(m, n, 16384, 5, 6).float().to(DEV)
+            z = (x.double() @ w.double() + b.double()).clamp(min=0)
+            want = z * keep + r.double()
+            tol = torch.finfo(t).eps / 2 * want.abs() + 2.0 ** -22 * (want.abs() + z * keep)
+            check(y, want.cpu(), tol.cpu(), off)
+
+
+@pytest.mark.parametrize("tname", TYPES)
+def test_relative_precision_of_activations(tname):
+    """Down their negative side, as far as the results are normal numbers.  The normal tail is a fit of 4e-7
+    (8.4e-6 for 16 bits, up to 6.5); an exponential's relative error is its exponent's absolute one, so it
+    grows with the exponent: z^2 / 2 has two roundings and a constant's (2.5 2^-24 of it), z log2 e one and a
+    constant's, and gelu_tanh's argument at most six more; 1 ulp for each of v_exp and v_rcp, 2^-24 for each of
+    up to four sums and products."""
+    t, few = TYPES[tname], 2 * 2.0 ** -23 + 4 * 2.0 ** -24
+    from dense_reference import act as f
+    one = torch.ones(1, 1, dtype=t, device=DEV)
+    for act, low in (("gelu", -12.0 if t == torch.float32 else -6.5), ("gelu_tanh", -9.0), ("silu", -80.0)):
+        x = torch.linspace(low, 0, 40001, dtype=torch.float64).to(t)[:, None]
+        z = x.double()
+        arg = {"gelu": 2.5 * z * z / 2, "silu": 1.5 * z.abs(),
+               "gelu_tanh": 8 * 2 * (2 / np.pi) ** 0.5 * (z.abs() + 0.044715 * z.abs() ** 3)}[act]
+        rel = few + 2.0 ** -24 * arg + (0 if act != "gelu" else 4e-7 if t == torch.float32 else 8.4e-6)
+        want = f(z, act)
+        tol = rel * want.abs()
+        tol = tol + torch.finfo(t).eps / 2 * (want.abs() + tol) + torch.finfo(t).smallest_normal * torch.finfo(t).eps
+        check(dgprf.linear(x.to(DEV), one, activation=act), want, tol, act)
 
 
 @pytest.mark.parametrize("tname", TYPES)
