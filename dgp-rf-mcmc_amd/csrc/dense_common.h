@@ -35,10 +35,12 @@ inline int elem_size(int dtype) { return dtype == DGPRF_F32 ? 4 : 2; }
 // precision (no 1 - erf cancellation).  Both forms are own least-squares fits, reweighted towards the
 // smallest maximal relative error.
 //  * fp32: e^{-a^2 / 2} Q(a), Q(a) = erfcx(a / sqrt 2) / 2 = t (c0 + c1 t + ... + c8 t^8), t = 1 / (1 + 0.35 a),
-//    a in [0, 14]: 3.2e-8 (4e-7 as evaluated in 32 bits).
+//    a in [0, 14]: 3.2e-8 (4e-7 as evaluated in 32 bits, without gauss()'s own error).
 //  * 16-bit types (whose rounding is 2^-12 and more): 2^{p(a)}, p of degree 7 fitted to log2 of the tail
 //    for a in [0, 6.5]: 8.3e-6 as evaluated, falling to 0 beyond; two instructions in three of the other.
-__device__ __forceinline__ float exp_of(float x) {  // e^x: v_exp_f32 is 2^x to 1 ulp
+// e^x: v_exp_f32 is 2^x to 1 ulp; the product's rounding is an absolute error of the exponent, so the relative
+// one grows with it, 1.5 2^-24 |x| (1.8e-6 at silu's z = -20; gauss() has 2.5 2^-24 z^2 / 2)
+__device__ __forceinline__ float exp_of(float x) {
   return __builtin_amdgcn_exp2f(x * 1.4426950408889634f);
 }
 __device__ __forceinline__ float gauss(float z) {  // e^{-z^2 / 2}

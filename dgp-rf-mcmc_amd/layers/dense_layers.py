@@ -1,9 +1,12 @@
-"""DenseLayer and DropoutLayer: layers trained by gradient, for the networks around the random-feature
-layers — a feature extractor below a DGP, the deterministic or MC-dropout network beside it.
+"""DenseLayer and DropoutLayer: layers trained by gradient, for the networks beside the random-feature
+ones — the deterministic or MC-dropout network that a DGP is compared with, or features trained by it.
 
 They call dgprf.linear / dgprf.dropout (one kernel for product, bias, activation, dropout and residual)
 and are differentiable: torch.autograd.grad(loss, layer.trainable_variables) and
-experiments.optimizers.Adam.apply_gradients train them.  The product is GPLayer's (X W, W [in, out]).
+experiments.optimizers.Adam.apply_gradients train them (16-bit weights with values and moments in 32
+bits).  RBFLayer, ARCLayer and GPLayer take their results as inputs but pass no gradient back: what they
+return has no autograd graph, so a DenseLayer in front of them is not trained through them.  The product
+is GPLayer's (X W, W [in, out]).
 """
 import torch
 

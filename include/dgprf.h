@@ -403,8 +403,8 @@ int dgprf_mass_estimate(const dgprf_plan_t *plan, const float *mean, const float
                         float *hmass_est, void *stream);
 
 /* ---------------- dense operators ---------------- */
-/* A dense layer and dropout, forward and backward, for networks around the random-feature layers
- * (feature extractors, deterministic and MC-dropout baselines).  x W is GPLayer's product
+/* A dense layer and dropout, forward and backward, for networks beside the random-feature layers
+ * (deterministic and MC-dropout baselines).  x W is GPLayer's product
  * (layers/GP_weight_layers.py:13), W [k][n] in its layout.
  *
  *   z = x W + b        y = r + s m a(z)        dropout:  y = r + s m x
