@@ -27,6 +27,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/library.h>
 
 #include "../../include/dgprf.h"
@@ -347,12 +348,19 @@ Tensor dropout_call(const Tensor& x, const Tensor& res, const Drop& drop) {
   return y;
 }
 
-// A gradient of these gradients would leave terms out silently: it is an error instead.
-variable_list once(variable_list grads, const char* what) {
-  if (!at::GradMode::is_enabled()) return grads;
-  const auto error = std::make_shared<torch::autograd::DelayedError>(
-      std::string("dgprf: ") + what + " has no second derivative", (int64_t)grads.size());
-  return (*error)(std::move(grads));
+// A gradient of these gradients would leave terms out silently: it is an error instead, on every path from
+// them to what the backward pass is of (the current node's inputs) and to the gradient dy that it got.
+void once(const Tensor& dy, const variable_list& grads, const char* what) {
+  if (!at::GradMode::is_enabled()) return;
+  torch::autograd::edge_list to;
+  if (const auto node = torch::autograd::get_current_node())
+    for (const auto& edge : node->next_edges())
+      if (edge.is_valid()) to.push_back(edge);
+  if (dy.requires_grad()) to.push_back(torch::autograd::impl::gradient_edge(dy));
+  const auto error = std::make_shared<torch::autograd::Error>(
+      std::string("dgprf: ") + what + " has no second derivative", std::move(to));
+  for (const Tensor& g : grads)
+    if (g.defined()) torch::autograd::set_history(g, error);
 }
 
 bool capturing(hipStream_t s) {  // (the null stream cannot be captured, and must not be asked while another is)
@@ -441,7 +449,8 @@ struct LinearFunction : public torch::autograd::Function<LinearFunction> {
                "dgprf_linear_backward");
     }
     const Tensor none;
-    return once({dx, dw, db, want_r ? grads[0] : none, none, none, none, none, none}, "linear");
+    once(grads[0], {dx, dw, db}, "linear");
+    return {dx, dw, db, want_r ? grads[0] : none, none, none, none, none, none};
   }
 };
 
@@ -466,7 +475,8 @@ struct DropoutFunction : public torch::autograd::Function<DropoutFunction> {
       dx = dropout_call(dy, Tensor(), Drop(args[0], args[1], args[2], step, dy));
     }
     const Tensor none;
-    return once({dx, args[3] && ctx->needs_input_grad(1) ? grads[0] : none, none, none, none, none}, "dropout");
+    once(grads[0], {dx}, "dropout");
+    return {dx, args[3] && ctx->needs_input_grad(1) ? grads[0] : none, none, none, none, none};
   }
 };
 

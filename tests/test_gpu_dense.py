@@ -730,6 +730,26 @@ def test_captured_masks_are_drawn_on_each_replay():
     assert not any(torch.equal(masks[i], masks[j]) for i, j in ((0, 1), (0, 2), (1, 2)))
 
 
+def test_second_derivatives_refused():
+    """A gradient made with create_graph carries the error, with a residual and without, so a penalty on it
+    does not lose its gradient silently; the gradient itself is the ordinary one."""
+    x, w = torch.ones(8, 8, device=DEV, requires_grad=True), torch.ones(8, 8, device=DEV, requires_grad=True)
+    b = torch.ones(8, device=DEV, requires_grad=True)
+    for op, leaf in ((lambda: dgprf.linear(x, w, b, "gelu"), x), (lambda: dgprf.linear(x, w, b), w),
+                     (lambda: dgprf.linear(x, w, b, "silu"), b), (lambda: dgprf.linear(x, w, residual=x), x),
+                     (lambda: dgprf.dropout(x, 0.5, seed=1, sub=2), x), (lambda: dgprf.dropout(w, 0.5, residual=x), w)):
+        y = op()
+        for top in (y.sum(), y.square().sum()):
+            want, = torch.autograd.grad(top, leaf, retain_graph=True)
+            g, = torch.autograd.grad(top, leaf, create_graph=True)
+            assert g.requires_grad and torch.equal(g, want)
+            with pytest.raises(RuntimeError, match="no second derivative"):
+                torch.autograd.grad(g.square().sum() + leaf.sum(), leaf)
+    # the residual's gradient is the incoming one, with its own derivative
+    g, = torch.autograd.grad(dgprf.dropout(w, 0.5, residual=x).square().sum(), x, create_graph=True)
+    assert bool((torch.autograd.grad(g.sum(), x)[0] == 2).all())
+
+
 @pytest.mark.parametrize("reentrant", [False, True])
 def test_activation_checkpointing(reentrant):
     """A recomputed forward pass makes the masks that are given, and the same gradients; it does not draw
