@@ -268,10 +268,12 @@ void no_tangent(const OptT& t, const char* what) {
   if (t.has_value()) no_tangent(*t, what);
 }
 
+// t with the values that its memory holds: the imaginary part of a conjugate is a view that is marked as negated
+Tensor plain(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
 // [..., n] as a matrix that the kernels can read: unit stride within a row, rows apart by 0 or by n and
 // more.  A view where the strides allow one.
 Tensor rows_of(const Tensor& t, int64_t n) {
-  const Tensor m = t.dim() == 2 ? t : t.reshape({-1, n});
+  const Tensor m = plain(t.dim() == 2 ? t : t.reshape({-1, n}));
   const bool ok = (n <= 1 || m.stride(1) == 1) &&
                   (m.size(0) <= 1 || m.stride(0) == 0 || m.stride(0) >= n);
   return ok ? m : m.contiguous();
@@ -502,7 +504,7 @@ Tensor linear(const Tensor& x, const Tensor& weight, const OptT& bias, int64_t a
   if (given(b)) {
     dense_like(*b, x, "bias");
     TORCH_CHECK_VALUE(b->dim() == 1 && b->size(0) == n, "dgprf: bias must be [", n, "], got ", b->sizes());
-    b = b->contiguous();
+    b = plain(b->contiguous());
   }
   if (given(r)) {
     dense_like(*r, x, "residual");

@@ -388,6 +388,22 @@ def test_strides(m, tname):
     both(base[:, 3:3 + k], wide[:k, 5:5 + n], dy, dy)
 
 
+def test_negated_views():
+    """The imaginary part of a conjugate is a view of the other sign's memory: its values count."""
+    g = _gen(14)
+    ones = [torch.complex(normal(g, *s), normal(g, *s)).to(DEV).conj().imag for s in ((6, 1), (1, 9), (9,), (6, 9), (6, 9))]
+    ones += [torch._neg_view(normal(g, *s).to(DEV)) for s in ((6, 8), (8, 9), (9,), (6, 9), (6, 9))]
+    for views in (ones[:5], ones[5:]):
+        assert all(v.is_neg() for v in views)
+        for args in (views, [v.clone() for v in views]):
+            leaf = [v.detach().requires_grad_() for v in args[:4]]
+            y = dgprf.linear(*leaf[:3], "silu", leaf[3], 0.25, 1, 2)
+            z = dgprf.dropout(args[0], 0.25, residual=args[0], seed=1, sub=2)
+            got = (y, z, *torch.autograd.grad(y, leaf, args[4]))
+            want = got if args is views else want
+            assert all(torch.equal(u, v) for u, v in zip(got, want))
+
+
 def test_leading_dimensions_and_no_rows():
     g = _gen(4)
     x, w = normal(g, 3, 5, 16).to(DEV).requires_grad_(), normal(g, 16, 24).to(DEV).requires_grad_()
