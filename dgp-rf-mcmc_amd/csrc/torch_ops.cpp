@@ -370,9 +370,11 @@ bool capturing(hipStream_t s) {  // (the null stream cannot be captured, and mus
   return s && hipStreamIsCapturing(s, &status) == hipSuccess && status == hipStreamCaptureStatusActive;
 }
 // A leaf that an earlier, living autograd graph uses has its accumulation on that graph's stream, and so has
-// every node of that graph.  The engine would make that stream wait for the captured one, which ends the
-// capture and then the process; called in a backward pass, before anything is enqueued.  Looks at all that
-// this pass still has to run behind the current node: a leaf may stand behind views and copies of it.
+// every node of that graph.  The engine makes that stream wait for the captured one: another stream joins the
+// capture by that (torch.cuda.make_graphed_callables' warm-up leaves such a graph), but the null stream
+// cannot, which ends the capture and then the process.  Called in a backward pass, before anything is
+// enqueued.  Looks at all that this pass still has to run behind the current node: a leaf may stand behind
+// views and copies of it.
 void check_capture(const char* what) {
   if (!capturing(c10::hip::getCurrentHIPStream().stream())) return;
   const auto current = torch::autograd::get_current_node();
@@ -387,9 +389,9 @@ void check_capture(const char* what) {
       if (!next || !node->task_should_compute_output(i) || !seen.insert(next).second) continue;
       if (const auto s = next->stream()) {
         const c10::Stream h(c10::Stream::UNSAFE, c10::Device(c10::DeviceType::HIP, s->device_index()), s->id());
-        TORCH_CHECK(capturing(c10::hip::HIPStream(c10::hip::HIPStream::UNCHECKED, h).stream()), "dgprf: ", what,
-                    ": this backward pass is being captured while an autograd graph from before the capture holds one "
-                    "of its leaves; delete that graph's results first");
+        TORCH_CHECK(c10::hip::HIPStream(c10::hip::HIPStream::UNCHECKED, h).stream(), "dgprf: ", what,
+                    ": this backward pass is being captured while an autograd graph from before the capture, on the "
+                    "default stream, holds one of its leaves; delete that graph's results first");
       }
       open.push_back(next);
     }

@@ -603,6 +603,34 @@ def test_capture_beside_an_eager_graph_of_a_viewed_leaf():
         del y
 
 
+def test_graphed_module():
+    """Forward and backward captured apart by torch.cuda.make_graphed_callables, inputs and weights behind
+    views: every replay has the eager results."""
+    g = _gen(15)
+
+    class Block(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.w = torch.nn.Parameter(normal(g, 56, 24, scale=0.2))
+            self.b = torch.nn.Parameter(normal(g, 56))
+
+        def forward(self, x):
+            return dgprf.linear(x, self.w.t(), self.b, "silu", dropout=0.2, seed=1, sub=2)
+
+    block, sample = Block().to(DEV), normal(g, 2, 5, 24).to(DEV).requires_grad_()
+    cases = []
+    for _ in range(3):
+        x, dy = normal(g, 2, 5, 24).to(DEV).requires_grad_(), normal(g, 2, 5, 56).to(DEV)
+        y = block(x)
+        cases.append((x, dy, y.detach(), torch.autograd.grad(y, (x, *block.parameters()), dy)))
+        del y
+    graphed = torch.cuda.make_graphed_callables(block, (sample,))
+    for x, dy, y, want in cases:
+        z = graphed(x)
+        got = torch.autograd.grad(z, (x, *block.parameters()), dy)
+        assert torch.equal(z, y) and all(torch.equal(u, v) for u, v in zip(got, want))
+
+
 def test_two_graphs_and_streams():
     """Two captured calls do not share scratch, and a call on another stream is ordered there."""
     g = _gen(8)
